@@ -234,7 +234,7 @@ def _plain_plan(s):
     req = req.clamp(max=new.numel() - 1)
     pos = cached[req] + t - q_starts[req]
     slot = table[req, (pos // page).clamp(max=stride - 1).long()] * page + pos % page
-    status = torch.stack([torch.where(ok, end, 0).max(), (~ok).sum()]).int()
+    status = torch.stack([torch.where(ok & (take > 0), end, 0).max(), (~ok).sum()]).int()
     return dict(table=table, q_starts=q_starts, kv_lens=cached + torch.where(ok, new, 0),
                 slots=torch.where(real & ok[req], slot, -1), positions=torch.where(real, pos, 0), status=status)
 
@@ -432,12 +432,13 @@ def _exact_plan(s):
     page = s["case"]["page"]
     cached, new, free = (s[k].tolist() for k in ("cached", "new", "free"))
     table = s["table"].cpu().numpy().copy()
-    tokens, left, taken, refused = s["slots"].numel(), s["free_count"].item(), 0, 0
+    tokens, left, asked, taken, refused = s["slots"].numel(), s["free_count"].item(), 0, 0, 0
     slots, positions = np.full(tokens, -1, np.int32), np.zeros(tokens, np.int32)
     starts, kv = [0], []
     for b, (c, n) in enumerate(zip(cached, new)):
         held, need = -(-c // page), -(-(c + n) // page)
-        good = need <= table.shape[1] and (need == held or taken + need - held <= left)
+        asked += need - held if need <= table.shape[1] else 0
+        good = need <= table.shape[1] and (need == held or asked <= left)
         for j in range(held, need if good else held):
             table[b, j] = free[taken]
             taken += 1
