@@ -189,6 +189,16 @@ int mdlc_ctx_create(int device, mdlc_ctx** out);
 int mdlc_ctx_destroy(mdlc_ctx* ctx);
 const char* mdlc_last_error(mdlc_ctx* ctx);
 int mdlc_get_stream(mdlc_ctx* ctx, void** stream); /* cudaStream_t of the context */
+/* Issues the context's later compute work (kernels, transfers that name no
+ * stream, memsets, events) on a cudaStream_t of the caller's instead of the
+ * context's own compute stream, so that buffers a host framework fills or
+ * reads on its stream need no extra ordering; `stream` may be null (the legacy
+ * default stream). The new stream first waits for what the context has issued
+ * so far. The caller's stream must outlive its use here: unbind (which makes the
+ * own stream wait in the same way) or bind another before destroying it.
+ * Rejected while a graph is being captured. */
+int mdlc_bind_stream(mdlc_ctx* ctx, void* stream);
+int mdlc_unbind_stream(mdlc_ctx* ctx);
 
 /* ---- memory (the C side owns device and pinned host allocations) ------- */
 int mdlc_alloc(mdlc_ctx* ctx, size_t bytes, void** dev);
@@ -373,6 +383,122 @@ typedef struct {
 } mdlc_se_desc;
 int mdlc_se_fc(mdlc_ctx* ctx, const mdlc_se_desc* desc, const void* pooled, const float* w1, const float* b1,
                const float* w2t, const float* b2, void* gate);
+
+/* ---- paged decoder operators -------------------------------------------
+ * One step of a decoder that answers requests from a paged key / value cache.
+ * No counterpart in the reference. A cache is
+ * [pages][kv_heads][page][head_dim] in the operators' type, so that one page of
+ * one head is contiguous; a slot is page_id * page + offset. Request b's new
+ * tokens are rows q_starts[b] .. q_starts[b + 1] - 1 of the packed token axis, and
+ * its cache pages the ids in row b of a block table [batch][table_stride].
+ * Lengths, tables and slots live on the device and are read by the kernels, so a
+ * captured step replays with new ones; the host gives upper bounds. Ids, slots
+ * and positions read on the device are checked: one outside its range is
+ * skipped and records MDLC_DEVERR_BOUNDS in the error word. */
+#define MDLC_MAX_REQUESTS 8192
+
+/* Block tables, slot maps and positions from request lengths. Request b holds
+ * cached_lens[b] tokens, so its first ceil(cached / page) table entries are
+ * page ids, and brings new_lens[b] more. Pages for them are taken from
+ * free_list in request order (the first *free_count entries, all free_pages
+ * when free_count is null) and appended to its row of block_table; other
+ * entries are left as they are. A request that would need more than
+ * table_stride entries or more pages than are left is refused: its row keeps its
+ * entries, its slots are -1 and kv_lens[b] stays cached_lens[b] (the pages that
+ * it would have taken are then not given to later requests either).
+ * q_starts[batch + 1]: running sums of new_lens, at most `tokens`; kv_lens[b]
+ * = cached + new; slots[tokens], positions[tokens]: each new token's slot and its
+ * index in its request; rows past the last request's get slot -1, position 0.
+ * status[0]: pages taken from the list; status[1]: requests refused. Negative
+ * lengths count as 0. Outputs must not overlap inputs; called again on the
+ * same inputs it gives the same outputs. */
+typedef struct {
+  int32_t batch;        /* requests, 1 .. MDLC_MAX_REQUESTS */
+  int32_t page;         /* tokens per page, 1 .. 1024 */
+  int32_t table_stride; /* entries per row of the block table */
+  int32_t tokens;       /* rows of slots and positions */
+  int32_t free_pages;   /* entries of free_list */
+} mdlc_page_desc;
+int mdlc_page_plan(mdlc_ctx* ctx, const mdlc_page_desc* desc, const int32_t* cached_lens, const int32_t* new_lens,
+                   const int32_t* free_list, const int32_t* free_count, int32_t* block_table, int32_t* q_starts,
+                   int32_t* kv_lens, int32_t* slots, int32_t* positions, int32_t* status);
+
+/* Rotary positions on queries and keys, and the keys and values written to
+ * their cache slots. The first rot_dim elements of a head are rot_dim / 2 pairs,
+ * (i, i + rot_dim / 2) or with `interleaved` (2i, 2i + 1); pair i belongs to
+ * one of `axes` position axes (section[a] pairs each, in order: time, height,
+ * width for images and video, one axis for text) and turns by the angle whose
+ * cosine and sine are table[positions[axis][t]][i]:
+ *   x' = x cos - y sin,  y' = y cos + x sin     (fp32, rounded once)
+ * The rest of the head passes unchanged. positions: [axes][tokens] in
+ * [0, max_pos); table: [max_pos][rot_dim / 2][2] fp32. q, k, v and q_out hold
+ * [tokens][heads][head_dim] with a stride between tokens each (slices of one
+ * packed projection, for instance); q_out may be q itself. A token whose slot is
+ * negative is padding: its q_out is written, the caches are not. q_out null:
+ * only the caches are written. */
+typedef struct {
+  int32_t tokens, heads, kv_heads, head_dim;
+  int32_t rot_dim;     /* even, <= head_dim */
+  int32_t interleaved; /* 0 or 1 */
+  int32_t axes;        /* 1 .. 4 */
+  int32_t section[4];  /* pairs of each axis; they sum to rot_dim / 2 */
+  int32_t max_pos;     /* rows of the table */
+  int32_t page, pages; /* tokens per page; pages of the caches */
+  int32_t dtype;       /* MDLC_BF16 or MDLC_F32 */
+  int64_t q_stride, k_stride, v_stride, out_stride; /* elements between tokens */
+} mdlc_rope_desc;
+int mdlc_rope_append(mdlc_ctx* ctx, const mdlc_rope_desc* desc, const void* q, const void* k, const void* v,
+                     const int32_t* positions, const float* table, const int32_t* slots, void* q_out, void* k_cache,
+                     void* v_cache);
+
+/* Attention of each request's new tokens over its cache pages. With i the
+ * token's index among its request's q_len new ones, it stands at position
+ * p = kv_lens[b] - q_len + i and sees key j when
+ *   j <= p and (window == 0 or j > p - window or j < sinks),
+ *   out = sum_j exp(s_j - lse) v_j,  s_j = scale q . k_j,  lse = log sum_j exp(s_j);
+ * a token that sees no key gets out = 0, lse = -inf. Heads e * G .. e * G + G - 1
+ * (G = heads / kv_heads) read key head e. fp32 scores, sums and statistics (lse is
+ * optional, [tokens][heads] fp32, may be null). Table entries of pages that no new
+ * token sees (behind the window, past kv_lens) are not read. A page id
+ * outside [0, pages) among the read ones counts as hidden keys. Keys and values
+ * past kv_lens may hold anything, NaN included. Rows past q_starts[batch] are left
+ * as they are. `workspace`: mdlc_paged_attn_workspace bytes, 16-byte aligned, for
+ * this call alone. q, out and caches are 16-byte aligned, the strides multiples of 8
+ * elements. max_q and max_kv bound every request's q_len and kv_len: longer ones
+ * are cut to them (kv_len also to table_stride * page). */
+typedef struct {
+  int32_t batch;   /* 1 .. MDLC_MAX_REQUESTS */
+  int32_t tokens;  /* rows of q and out */
+  int32_t heads, kv_heads;
+  int32_t head_dim; /* a multiple of 8, 8 .. 128 */
+  int32_t page, pages, table_stride;
+  int32_t max_q, max_kv;
+  int32_t window, sinks; /* window 0: none (sinks is then without effect) */
+  int32_t dtype;         /* MDLC_BF16 or MDLC_F32 */
+  float scale;
+  int64_t q_stride, out_stride; /* elements between tokens */
+} mdlc_attn_desc;
+int mdlc_paged_attn_workspace(const mdlc_attn_desc* desc, size_t* bytes);
+int mdlc_paged_attn(mdlc_ctx* ctx, const mdlc_attn_desc* desc, const void* q, const void* k_cache, const void* v_cache,
+                    const int32_t* block_table, const int32_t* q_starts, const int32_t* kv_lens, void* out, float* lse,
+                    void* workspace);
+
+/* Products of a few rows with 4-bit weights:
+ *   y[i][o] = bias[o] + sum_c x[i][c] (code[o][c] - zero[o][c / group]) scale[o][c / group]
+ * codes: [n][k / 2] bytes, column c in the low (c even) or high (c odd) nibble of
+ * byte c / 2; scales: [n][k / group] bf16; zeros: [n][k / group] uint8 0..15, null:
+ * 8; bias: [n] fp32 or null. Products are exact, sums in fp32 (an fp32 x is taken
+ * as three bf16 parts). codes 16-byte aligned; x 16-byte aligned with x_stride a multiple of 8. */
+typedef struct {
+  int32_t m;     /* rows; made for 1 .. 32, more re-read the weights */
+  int32_t n;     /* output columns */
+  int32_t k;     /* a multiple of group */
+  int32_t group; /* 32, 64 or 128 */
+  int32_t x_type, y_type; /* MDLC_BF16 or MDLC_F32 */
+  int64_t x_stride, y_stride; /* elements between rows */
+} mdlc_w4_desc;
+int mdlc_gemv_w4(mdlc_ctx* ctx, const mdlc_w4_desc* desc, const void* x, const uint8_t* codes, const void* scales,
+                 const uint8_t* zeros, const float* bias, void* y);
 
 /* ---- CUDA graph capture of a whole run (b=1 latency) ------------------- */
 int mdlc_graph_begin(mdlc_ctx* ctx);

@@ -28,6 +28,7 @@ F32, BF16, S8, U8, S32 = 0, 1, 2, 3, 4
  EW_RELU, EW_CLIP, EW_SIGMOID, EW_TANH, EW_LEAKY_RELU, EW_HARD_SIGMOID, EW_HARD_SWISH, EW_ERF,
  EW_GELU, EW_MAX, EW_MIN) = range(21)
 EW_MAX_INPUTS, EW_MAX_OUTPUTS, EW_MAX_INSTR = 4, 2, 24
+MAX_REQUESTS = 8192
 BC_FULL, BC_NC, BC_C, BC_SCALAR = 0, 1, 2, 3
 
 ELEM_BYTES = {F32: 4, BF16: 2, S8: 1, U8: 1, S32: 4}
@@ -103,6 +104,27 @@ class SeDesc(C.Structure):
                 ("hw", C.c_int32)]
 
 
+class PageDesc(C.Structure):
+    _fields_ = [(f, C.c_int32) for f in ("batch", "page", "table_stride", "tokens", "free_pages")]
+
+
+class RopeDesc(C.Structure):
+    _fields_ = [(f, C.c_int32) for f in ("tokens", "heads", "kv_heads", "head_dim", "rot_dim", "interleaved", "axes")] + \
+        [("section", C.c_int32 * 4)] + [(f, C.c_int32) for f in ("max_pos", "page", "pages", "dtype")] + \
+        [(f, C.c_int64) for f in ("q_stride", "k_stride", "v_stride", "out_stride")]
+
+
+class AttnDesc(C.Structure):
+    _fields_ = [(f, C.c_int32) for f in ("batch", "tokens", "heads", "kv_heads", "head_dim", "page", "pages",
+                                         "table_stride", "max_q", "max_kv", "window", "sinks", "dtype")] + \
+        [("scale", C.c_float), ("q_stride", C.c_int64), ("out_stride", C.c_int64)]
+
+
+class W4Desc(C.Structure):
+    _fields_ = [(f, C.c_int32) for f in ("m", "n", "k", "group", "x_type", "y_type")] + \
+        [("x_stride", C.c_int64), ("y_stride", C.c_int64)]
+
+
 # exported symbol -> (argtypes, restype); the CPU test suite checks every
 # function declared in include/mdlc_b200.h is exported and listed here.
 _P, _I, _S = C.c_void_p, C.c_int, C.c_size_t
@@ -113,6 +135,8 @@ SIGNATURES = {
     "mdlc_ctx_destroy": ([_P], C.c_int),
     "mdlc_last_error": ([_P], C.c_char_p),
     "mdlc_get_stream": ([_P, C.POINTER(C.c_void_p)], C.c_int),
+    "mdlc_bind_stream": ([_P, _P], C.c_int),
+    "mdlc_unbind_stream": ([_P], C.c_int),
     "mdlc_alloc": ([_P, _S, C.POINTER(C.c_void_p)], C.c_int),
     "mdlc_free": ([_P, _P], C.c_int),
     "mdlc_host_alloc": ([_P, _S, C.POINTER(C.c_void_p)], C.c_int),
@@ -146,6 +170,11 @@ SIGNATURES = {
     "mdlc_copy4d": ([_P, C.POINTER(CopyDesc), _P, _P], C.c_int),
     "mdlc_softmax": ([_P, C.POINTER(SoftmaxDesc), _P, _P], C.c_int),
     "mdlc_se_fc": ([_P, C.POINTER(SeDesc), _P, _P, _P, _P, _P, _P], C.c_int),
+    "mdlc_page_plan": ([_P, C.POINTER(PageDesc)] + [_P] * 10, C.c_int),
+    "mdlc_rope_append": ([_P, C.POINTER(RopeDesc)] + [_P] * 9, C.c_int),
+    "mdlc_paged_attn_workspace": ([C.POINTER(AttnDesc), C.POINTER(C.c_size_t)], C.c_int),
+    "mdlc_paged_attn": ([_P, C.POINTER(AttnDesc)] + [_P] * 9, C.c_int),
+    "mdlc_gemv_w4": ([_P, C.POINTER(W4Desc)] + [_P] * 6, C.c_int),
     "mdlc_graph_begin": ([_P], C.c_int),
     "mdlc_graph_end": ([_P], C.c_int),
     "mdlc_graph_launch": ([_P], C.c_int),
@@ -325,6 +354,32 @@ class Context:
                                        C.c_void_p(b1 or None), C.c_void_p(w2t), C.c_void_p(b2 or None),
                                        C.c_void_p(gate)), "se_fc")
 
+    # the paged decoder operators take device addresses as plain integers (0: none)
+    # and go straight to the library: a decode step calls them often
+    def page_plan(self, desc: PageDesc, cached_lens, new_lens, free_list, free_count, block_table, q_starts, kv_lens,
+                  slots, positions, status) -> None:
+        st = self.lib.mdlc_page_plan(self.h, desc, cached_lens, new_lens, free_list, free_count, block_table, q_starts,
+                                     kv_lens, slots, positions, status)
+        if st:
+            self.check(st, "page_plan")
+
+    def rope_append(self, desc: RopeDesc, q, k, v, positions, table, slots, q_out, k_cache, v_cache) -> None:
+        st = self.lib.mdlc_rope_append(self.h, desc, q, k, v, positions, table, slots, q_out, k_cache, v_cache)
+        if st:
+            self.check(st, "rope_append")
+
+    def paged_attn(self, desc: AttnDesc, q, k_cache, v_cache, block_table, q_starts, kv_lens, out, lse,
+                   workspace) -> None:
+        st = self.lib.mdlc_paged_attn(self.h, desc, q, k_cache, v_cache, block_table, q_starts, kv_lens, out, lse,
+                                      workspace)
+        if st:
+            self.check(st, "paged_attn")
+
+    def gemv_w4(self, desc: W4Desc, x, codes, scales, zeros, bias, y) -> None:
+        st = self.lib.mdlc_gemv_w4(self.h, desc, x, codes, scales, zeros, bias, y)
+        if st:
+            self.check(st, "gemv_w4")
+
     def to_nhwc(self, x, n, c, h, w, y, cs, dtype, inv_scale=1.0, zp=0) -> None:
         self.check(self.lib.mdlc_nchw_to_nhwc(self.h, C.c_void_p(x), n, c, h, w, C.c_void_p(y), cs, dtype,
                                               C.c_float(inv_scale), zp), "nchw_to_nhwc")
@@ -371,6 +426,13 @@ class Context:
         self.check(self.lib.mdlc_get_stream(self.h, C.byref(s)), "get_stream")
         return s.value or 0
 
+    def bind_stream(self, stream: int) -> None:
+        """Issue later compute work on the caller's ``cudaStream_t`` (0: the legacy default stream)."""
+        self.check(self.lib.mdlc_bind_stream(self.h, C.c_void_p(stream)), "bind_stream")
+
+    def unbind_stream(self) -> None:
+        self.check(self.lib.mdlc_unbind_stream(self.h), "unbind_stream")
+
     def timeout_probe(self, limit_us: int) -> None:
         self.check(self.lib.mdlc_debug_timeout_probe(self.h, int(limit_us)), "timeout_probe")
 
@@ -393,6 +455,15 @@ class Context:
             self.close()
         except Exception:
             pass
+
+
+def paged_attn_workspace(desc: AttnDesc) -> int:
+    """Bytes of the workspace that ``Context.paged_attn`` wants for ``desc``."""
+    n = C.c_size_t(0)
+    st = load().mdlc_paged_attn_workspace(C.byref(desc), C.byref(n))
+    if st != OK:
+        raise MdlcError(st, "paged_attn_workspace: unsupported descriptor")
+    return n.value
 
 
 def weight_bytes(desc: ConvDesc) -> int:

@@ -53,7 +53,8 @@ int mdlc_ctx_create(int device, mdlc_ctx** out) {
   mdlc_ctx* ctx = new mdlc_ctx();
   ctx->device = device;
   ctx->num_sms = prop.multiProcessorCount;
-  if (cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking) != cudaSuccess ||
+  if (cudaStreamCreateWithFlags(&ctx->own_stream, cudaStreamNonBlocking) != cudaSuccess ||
+      cudaEventCreateWithFlags(&ctx->order, cudaEventDisableTiming) != cudaSuccess ||
       cudaStreamCreateWithFlags(&ctx->copy_stream, cudaStreamNonBlocking) != cudaSuccess ||
       cudaMalloc(&ctx->d_err, 256) != cudaSuccess ||
       cudaMemset(ctx->d_err, 0, 256) != cudaSuccess || cudaMalloc(&ctx->d_pad, 4096) != cudaSuccess ||
@@ -63,6 +64,7 @@ int mdlc_ctx_create(int device, mdlc_ctx** out) {
     delete ctx;
     return MDLC_ERR_CUDA;
   }
+  ctx->stream = ctx->own_stream;
   {
     uint8_t pat[4096];
     for (int i = 0; i < 4096; ++i) pat[i] = (uint8_t)(i >> 4);
@@ -80,7 +82,9 @@ int mdlc_ctx_create(int device, mdlc_ctx** out) {
 int mdlc_ctx_destroy(mdlc_ctx* ctx) {
   if (!ctx) return MDLC_OK;
   cudaSetDevice(ctx->device);
-  cudaStreamSynchronize(ctx->stream);
+  // a bound stream may be gone by now: wait for the device instead
+  if (ctx->bound) cudaDeviceSynchronize();
+  cudaStreamSynchronize(ctx->own_stream);
   if (ctx->copy_stream) cudaStreamSynchronize(ctx->copy_stream);
   if (ctx->graph_exec) cudaGraphExecDestroy(ctx->graph_exec);
   if (ctx->graph) cudaGraphDestroy(ctx->graph);
@@ -91,7 +95,8 @@ int mdlc_ctx_destroy(mdlc_ctx* ctx) {
   cudaFree(ctx->d_pad);
   cudaFree(ctx->d_split_ws);
   cudaFree(ctx->d_split_cnt);
-  cudaStreamDestroy(ctx->stream);
+  cudaEventDestroy(ctx->order);
+  cudaStreamDestroy(ctx->own_stream);
   if (ctx->copy_stream) cudaStreamDestroy(ctx->copy_stream);
   delete ctx;
   return MDLC_OK;
@@ -103,6 +108,28 @@ int mdlc_get_stream(mdlc_ctx* ctx, void** stream) {
   if (!ctx || !stream) return MDLC_ERR_INVALID;
   *stream = (void*)ctx->stream;
   return MDLC_OK;
+}
+
+static int switch_stream(mdlc_ctx* ctx, cudaStream_t to, bool bound) {
+  if (ctx->capturing) return mdlc_set_error(ctx, MDLC_ERR_INVALID, "the stream cannot change during a capture");
+  cudaSetDevice(ctx->device);
+  cudaError_t e = cudaEventRecord(ctx->order, ctx->stream);
+  if (e == cudaSuccess) e = cudaStreamWaitEvent(to, ctx->order, 0);
+  if (e != cudaSuccess) return mdlc_cuda_status(ctx, e, "bind stream");
+  ctx->stream = to;
+  ctx->bound = bound;
+  return MDLC_OK;
+}
+
+int mdlc_bind_stream(mdlc_ctx* ctx, void* stream) {
+  if (!ctx) return MDLC_ERR_INVALID;
+  return switch_stream(ctx, static_cast<cudaStream_t>(stream), true);
+}
+
+int mdlc_unbind_stream(mdlc_ctx* ctx) {
+  if (!ctx) return MDLC_ERR_INVALID;
+  if (!ctx->bound) return MDLC_OK;
+  return switch_stream(ctx, ctx->own_stream, false);
 }
 
 int mdlc_alloc(mdlc_ctx* ctx, size_t bytes, void** dev) {
@@ -239,10 +266,11 @@ int mdlc_graph_begin(mdlc_ctx* ctx) {
   if (!ctx) return MDLC_ERR_INVALID;
   cudaSetDevice(ctx->device);
   mdlc_graph_reset(ctx);
-  ctx->capturing = true;
+  // the legacy default stream (a bound one) cannot be captured: no capture is open then
+  const cudaError_t e = cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal);
+  ctx->capturing = e == cudaSuccess;
   ctx->captured_launches = 0;
-  return mdlc_cuda_status(
-      ctx, cudaStreamBeginCapture(ctx->stream, cudaStreamCaptureModeThreadLocal), "begin capture");
+  return mdlc_cuda_status(ctx, e, "begin capture");
 }
 
 int mdlc_graph_end(mdlc_ctx* ctx) {

@@ -16,7 +16,10 @@ static constexpr unsigned long long kWaitLimitNs = 2000000000ull;
 struct mdlc_ctx {
   int device = 0;
   int num_sms = 148;
-  cudaStream_t stream = nullptr;       // compute stream (every kernel)
+  cudaStream_t stream = nullptr;       // compute stream (every kernel): own_stream or a bound one
+  cudaStream_t own_stream = nullptr;
+  bool bound = false;                  // stream is a caller's
+  cudaEvent_t order = nullptr;         // orders the two when the binding changes
   cudaStream_t copy_stream = nullptr;  // host<->device transfers overlapped with compute
   int* d_err = nullptr;  // device error word (first failure wins)
   uint8_t* d_pad = nullptr;  // 256 x 16-byte fill patterns (byte value v at v*16)
