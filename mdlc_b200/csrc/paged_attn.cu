@@ -16,8 +16,7 @@
 //     over the blocks whatever the requests' lengths; a tile cut between blocks leaves
 //     partial sums in the workspace, which attn_join_kernel adds in block order.
 //   chunk mode (many rows): a block per row tile.
-#include "common.cuh"
-#include "runtime.h"
+#include "paged_attn.cuh"
 
 namespace mdlc {
 namespace {
@@ -27,56 +26,11 @@ constexpr int kStages = 3;
 constexpr int kUnit = 128;      // keys of one unit of split work
 constexpr int kMaxBlocks = 512; // split-mode blocks at most (bounds the workspace)
 constexpr int kJoinThreads = 256;
-
-struct AttnArgs {
-  mdlc_attn_desc d;
-  const void *q, *k, *v;
-  const int32_t *table, *q_starts, *kv_lens;
-  void* out;
-  float* lse;
-  int group;          // query heads per key head
-  int split_rows;     // requests with at most this many rows go to split mode
-  float scale_log2;   // scale * log2(e)
-  // workspace: partial sums [slot][rows][hdp], their maxima and sums [slot][rows], first unit of each request
-  float *part_o, *part_m, *part_l;
-  long long* first_unit;  // [batch + 1]
-};
+constexpr int kLeastKeys = 256; // keys of a share of a chunk tile at least
+constexpr int kChunkBlocks = 148;  // shares are made until chunk mode fills this many SMs
 
 template <typename T, int HDP>
 constexpr int block_keys() { return sizeof(T) * HDP <= 256 ? 32 : 16; }
-
-// ------------------------------------------------------------ one request's geometry
-struct Request {
-  int q0, q_len, kv_len;
-};
-MDLC_DEV Request request_of(const AttnArgs& a, int b) {
-  Request r;
-  const int s0 = __ldg(a.q_starts + b), s1 = __ldg(a.q_starts + b + 1);
-  r.q0 = max(0, min(s0, a.d.tokens));
-  r.q_len = min(max(0, min(s1, a.d.tokens) - r.q0), a.d.max_q);
-  r.kv_len = max(0, min(__ldg(a.kv_lens + b), a.d.max_kv));  // the host has cut max_kv to the table's row
-  return r;
-}
-
-// Blocks of BT keys that the rows of tokens [i0, i1] of a request can see: blocks
-// [0, n_first) hold the first tokens kept by `sinks`, the others start at `start`.
-struct Span {
-  int lo, hi;     // keys below lo are hidden from every row unless below sinks; keys from hi on too
-  int n_first, start, n;
-};
-template <int BT>
-MDLC_DEV Span span_of(const AttnArgs& a, const Request& r, int i0, int i1) {
-  Span s;
-  const int shift = r.kv_len - r.q_len;
-  s.hi = max(0, min(r.kv_len, shift + i1 + 1));
-  s.lo = a.d.window > 0 ? (int)max(0ll, (long long)shift + i0 - a.d.window + 1) : 0;
-  s.n_first = (min(a.d.sinks, s.lo) + BT - 1) / BT;
-  s.start = s.lo / BT * BT;
-  if (s.start <= s.n_first * BT) s.n_first = s.start = 0;
-  s.n = s.n_first + (max(0, s.hi - s.start) + BT - 1) / BT;
-  if (s.hi == 0) s.n = 0;
-  return s;
-}
 
 // ------------------------------------------------------------ mma fragments
 MDLC_DEV void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -122,13 +76,6 @@ MDLC_DEV float quad_sum(float v) {
   v += __shfl_xor_sync(0xffffffffu, v, 1);
   return v + __shfl_xor_sync(0xffffffffu, v, 2);
 }
-
-template <typename T>
-MDLC_DEV void store_out(T* p, float v);
-template <>
-MDLC_DEV void store_out<float>(float* p, float v) { *p = v; }
-template <>
-MDLC_DEV void store_out<__nv_bfloat16>(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 // ------------------------------------------------------------ the kernel
 template <typename T, int HDP, int WM>
@@ -188,7 +135,7 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
       qa[ks][i] = (qp[i & 1] && c < d.head_dim) ? __ldg(reinterpret_cast<const uint32_t*>(qp[i & 1] + c)) : 0u;
     }
 
-  auto base_of = [&](int blk) { return blk < sp.n_first ? blk * BT : sp.start + (blk - sp.n_first) * BT; };
+  auto base_of = [&](int blk) { return key_of_block(sp, blk, BT); };
   // cache row (key `lane` of the block) or -1: hidden from every row, or no such page
   auto row_of = [&](int blk) {
     const int j = base_of(blk) + lane;
@@ -409,37 +356,11 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
   __syncthreads();  // the next piece takes the ring again
 }
 
-// exclusive sum over the block's threads of v; *total: the sum of all
-MDLC_DEV long long block_scan(long long v, long long* warp_sums, long long* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  long long run = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, run, o);
-    if (lane >= o) run += x;
-  }
-  if (lane == 31) warp_sums[warp] = run;
-  __syncthreads();
-  long long before = 0, all = 0;
-  for (int w = 0; w < nw; ++w) {
-    if (w < warp) before += warp_sums[w];
-    all += warp_sums[w];
-  }
-  __syncthreads();
-  *total = all;
-  return before + run - v;
-}
-
-struct Place {
-  int b;
-  long long first;  // first unit (split) or tile (chunk) of request b
-};
-
 // the block that holds unit u when `units` are cut into `blocks` runs [c units / blocks, (c + 1) units / blocks)
 MDLC_DEV int block_of(long long u, long long units, int blocks) { return (int)(((u + 1) * blocks - 1) / units); }
 
-template <typename T, int HDP, int WM, bool SPLIT>
-__global__ void __launch_bounds__(kAttnThreads) attn_kernel(const AttnArgs a, int* err) {
+template <typename T, int HDP, int WM>
+__global__ void __launch_bounds__(kAttnThreads) attn_split_kernel(const AttnArgs a, int* err) {
   using K = Cfg<T, HDP, WM>;
   constexpr int UB = kUnit / K::BT;
   extern __shared__ __align__(128) unsigned char attn_smem[];
@@ -449,48 +370,34 @@ __global__ void __launch_bounds__(kAttnThreads) attn_kernel(const AttnArgs a, in
   pdl_wait();
   pdl_trigger();
   const mdlc_attn_desc& d = a.d;
-  // units (split) or row tiles (chunk) of a request and key head
-  auto count_of = [&](int b) -> long long {
+  // units of a request and key head
+  auto units_of = [&](int b) -> long long {
     const Request r = request_of(a, b);
     const long long rows = (long long)r.q_len * a.group;
-    if constexpr (SPLIT) {
-      if (rows == 0 || rows > a.split_rows) return 0;
-      return max(1, (span_of<K::BT>(a, r, 0, r.q_len - 1).n + UB - 1) / UB);
-    } else {
-      if (rows <= a.split_rows) return 0;
-      return (rows + K::ROWS - 1) / K::ROWS;
-    }
+    if (rows == 0 || rows > a.split_rows) return 0;
+    return max(1, (span_of(a, r, 0, r.q_len - 1, K::BT).n + UB - 1) / UB);
   };
   const int per = (d.batch + kAttnThreads - 1) / kAttnThreads;
   const int b0 = min((int)threadIdx.x * per, d.batch), b1 = min(b0 + per, d.batch);
-  const int heads = SPLIT ? d.kv_heads : 1;  // key heads that share the line of work
   long long mine = 0, total;
-  for (int b = b0; b < b1; ++b) mine += count_of(b) * heads;
-  long long before = block_scan(mine, warp_sums, &total);
-  if (SPLIT && blockIdx.x == 0) {
+  for (int b = b0; b < b1; ++b) mine += units_of(b) * d.kv_heads;
+  const long long before = block_scan(mine, warp_sums, &total);
+  if (blockIdx.x == 0) {
     long long at = before;
     for (int b = b0; b < b1; ++b) {
       a.first_unit[b] = at;
-      at += count_of(b) * heads;
+      at += units_of(b) * d.kv_heads;
       if (b == d.batch - 1) a.first_unit[d.batch] = at;
     }
   }
-  long long u0, u1;
-  int blocks = 1;
-  if constexpr (SPLIT) {
-    blocks = (int)min((long long)gridDim.x, total);
-    if ((int)blockIdx.x >= blocks) return;
-    u0 = (long long)blockIdx.x * total / blocks;
-    u1 = (long long)(blockIdx.x + 1) * total / blocks;
-  } else {
-    if ((long long)blockIdx.x >= total) return;
-    u0 = total - 1 - blockIdx.x;  // the last tiles of a request see the most keys: first
-    u1 = u0 + 1;
-  }
+  const int blocks = (int)min((long long)gridDim.x, total);
+  if ((int)blockIdx.x >= blocks) return;
+  long long u0 = (long long)blockIdx.x * total / blocks;
+  const long long u1 = (long long)(blockIdx.x + 1) * total / blocks;
   if (u0 >= before && u0 < before + mine) {
     long long at = before;
     for (int b = b0;; ++b) {
-      const long long n = count_of(b) * heads;
+      const long long n = units_of(b) * d.kv_heads;
       if (u0 < at + n) {
         place_s = {b, at};
         break;
@@ -500,28 +407,81 @@ __global__ void __launch_bounds__(kAttnThreads) attn_kernel(const AttnArgs a, in
   }
   __syncthreads();
   Place pl = place_s;
-  if constexpr (SPLIT) {
-    while (u0 < u1) {
-      const Request rq = request_of(a, pl.b);
-      const long long n = count_of(pl.b);
-      if (u0 >= pl.first + n * heads) {
-        pl.first += n * heads;
-        ++pl.b;
-        continue;
-      }
-      const int e = (int)((u0 - pl.first) / n);
-      const long long tile0 = pl.first + e * n, end = min(u1, tile0 + n);
-      const Span sp = span_of<K::BT>(a, rq, 0, rq.q_len - 1);
-      const int blk0 = (int)(u0 - tile0) * UB, blk1 = min((int)(end - tile0) * UB, sp.n);
-      attn_piece<T, HDP, WM>(a, attn_smem, valid_s, err, pl.b, rq, e, 0, sp, blk0, blk1, u0 == tile0 && end == tile0 + n,
-                             (long long)pl.b * d.kv_heads + e + blockIdx.x);
-      u0 = end;
-    }
-  } else {
+  while (u0 < u1) {
     const Request rq = request_of(a, pl.b);
-    const int r0 = (int)(u0 - pl.first) * K::ROWS, rows = rq.q_len * a.group;
-    const Span sp = span_of<K::BT>(a, rq, r0 / a.group, (min(r0 + K::ROWS, rows) - 1) / a.group);
-    attn_piece<T, HDP, WM>(a, attn_smem, valid_s, err, pl.b, rq, blockIdx.y, r0, sp, 0, sp.n, true, 0);
+    const long long n = units_of(pl.b);
+    if (u0 >= pl.first + n * d.kv_heads) {
+      pl.first += n * d.kv_heads;
+      ++pl.b;
+      continue;
+    }
+    const int e = (int)((u0 - pl.first) / n);
+    const long long tile0 = pl.first + e * n, end = min(u1, tile0 + n);
+    const Span sp = span_of(a, rq, 0, rq.q_len - 1, K::BT);
+    const int blk0 = (int)(u0 - tile0) * UB, blk1 = min((int)(end - tile0) * UB, sp.n);
+    attn_piece<T, HDP, WM>(a, attn_smem, valid_s, err, pl.b, rq, e, 0, sp, blk0, blk1, u0 == tile0 && end == tile0 + n,
+                           (long long)pl.b * d.kv_heads + e + blockIdx.x);
+    u0 = end;
+  }
+}
+
+// a block per row tile (x), key head (y) and share of its keys (z)
+template <typename T, int HDP>
+__global__ void __launch_bounds__(kAttnThreads) attn_chunk_kernel(const AttnArgs a, int* err) {
+  using K = Cfg<T, HDP, 4>;
+  extern __shared__ __align__(128) unsigned char attn_smem[];
+  __shared__ uint32_t valid_s[K::WN][kStages];
+  __shared__ long long warp_sums[kAttnThreads / 32];
+  __shared__ Place place_s;
+  pdl_wait();
+  pdl_trigger();
+  Tile t;
+  if (!find_tile(a, blockIdx.x, K::ROWS, warp_sums, &place_s, &t)) return;
+  const Span sp = span_of(a, t.rq, t.r0 / a.group, (min(t.r0 + K::ROWS, t.rows) - 1) / a.group, K::BT);
+  const int ns = splits_of(a, sp.n, kLeastKeys / K::BT), z = blockIdx.z;
+  if (z >= ns) return;
+  attn_piece<T, HDP, 4>(a, attn_smem, valid_s, err, t.b, t.rq, blockIdx.y, t.r0, sp, (int)((long long)z * sp.n / ns),
+                        (int)((long long)(z + 1) * sp.n / ns), ns == 1,
+                        ((long long)blockIdx.x * a.d.kv_heads + blockIdx.y) * a.splits + z);
+}
+
+// Adds the shares of a chunk tile, in order. A warp per row.
+template <typename T, int HDP>
+__global__ void __launch_bounds__(kJoinThreads) attn_chunk_join_kernel(const AttnArgs a, int tile_rows, int bt) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int V = HDP / 32;
+  __shared__ long long warp_sums[kJoinThreads / 32];
+  __shared__ Place place_s;
+  Tile t;
+  if (!find_tile(a, blockIdx.x, tile_rows, warp_sums, &place_s, &t)) return;
+  const Span sp = span_of(a, t.rq, t.r0 / a.group, (min(t.r0 + tile_rows, t.rows) - 1) / a.group, bt);
+  const int ns = splits_of(a, sp.n, kLeastKeys / bt);
+  if (ns == 1) return;
+  const mdlc_attn_desc& d = a.d;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = blockIdx.y;
+  const long long slot0 = ((long long)blockIdx.x * d.kv_heads + e) * a.splits;
+  const int per = (tile_rows + gridDim.z - 1) / gridDim.z, rl0 = blockIdx.z * per;
+  for (int rl = rl0 + warp; rl < min(rl0 + per, min(tile_rows, t.rows - t.r0)); rl += kJoinThreads / 32) {
+    const int r = t.r0 + rl;
+    float top = -INFINITY, sum = 0.0f, acc[V] = {};
+    for (int s = 0; s < ns; ++s) top = fmaxf(top, a.part_m[(slot0 + s) * tile_rows + rl]);
+    const float safe = top == -INFINITY ? 0.0f : top;
+#pragma unroll 4
+    for (int s = 0; s < ns; ++s) {
+      const long long at = (slot0 + s) * tile_rows + rl;
+      const float f = exp2f(a.part_m[at] - safe);
+      sum = fmaf(f, a.part_l[at], sum);
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] = fmaf(f, a.part_o[at * HDP + i * 32 + lane], acc[i]);
+    }
+    const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+    const int tok = t.rq.q0 + r / a.group, head = e * a.group + r % a.group;
+    T* po = static_cast<T*>(a.out) + (long long)tok * d.out_stride + (long long)head * d.head_dim;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i * 32 + lane < d.head_dim) store_out<T>(po + i * 32 + lane, acc[i] * inv);
+    if (a.lse && lane == 0) a.lse[(long long)tok * d.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
   }
 }
 
@@ -613,11 +573,33 @@ int split_groups(const mdlc_attn_desc& d) {
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
+// chunk mode's geometry: which kernel, row tiles at most (full ones, and one more per request), shares per tile
+struct Chunk {
+  bool used, tc;
+  int rows, tiles, splits;
+};
+Chunk chunk_of(const mdlc_attn_desc& d) {
+  const int group = d.heads / d.kv_heads;
+  Chunk c = {};
+  c.used = (long long)d.max_q * group > 16 * split_groups(d);
+  c.tc = attn_tc_fits(d);
+  c.rows = c.tc ? kTcRows : 64;
+  c.tiles = (int)min((long long)d.tokens * group / c.rows + d.batch, (long long)INT32_MAX);
+  // the mma.sync kernel runs three blocks per SM
+  const long long room = kChunkBlocks * (c.tc ? 1 : 3) / ((long long)c.tiles * d.kv_heads);
+  c.splits = (int)max(1ll, min(room, min(16ll, (long long)d.max_kv / kLeastKeys)));
+  return c;
+}
+
 struct Layout {
   size_t part_o, part_m, part_l, first_unit, total;
 };
 Layout layout_of(const mdlc_attn_desc& d) {
-  const size_t slots = (size_t)d.batch * d.kv_heads + kMaxBlocks, rows = slots * 16 * split_groups(d);
+  const size_t slots = (size_t)d.batch * d.kv_heads + kMaxBlocks;
+  size_t rows = slots * 16 * split_groups(d);
+  const Chunk c = chunk_of(d);
+  // the two modes run one after the other and share the space
+  if (c.used && c.splits > 1) rows = max(rows, (size_t)c.tiles * d.kv_heads * c.splits * c.rows);
   Layout l;
   l.part_o = 0;
   l.part_m = align256(rows * padded_dim(d.head_dim) * 4);
@@ -642,37 +624,44 @@ const char* check_desc(const mdlc_attn_desc* d) {
   return nullptr;
 }
 
-template <typename T, int HDP, int WM, bool SPLIT>
-cudaError_t launch_attn(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid) {
-  const int smem = Cfg<T, HDP, WM>::SMEM;
-  auto* kern = attn_kernel<T, HDP, WM, SPLIT>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  mdlc_note_launch(ctx);
-  return launch_pdl(kern, grid, dim3(kAttnThreads), smem, ctx->stream, a, ctx->d_err);
-}
-
 template <typename T, int HDP, int WM>
 cudaError_t run_split(mdlc_ctx* ctx, const AttnArgs& a) {
+  const int smem = Cfg<T, HDP, WM>::SMEM;
+  auto* kern = attn_split_kernel<T, HDP, WM>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return e;
   // one or two blocks per SM, as shared memory allows
-  const int blocks = min(kMaxBlocks, ctx->num_sms * (Cfg<T, HDP, WM>::SMEM <= 100 * 1024 ? 2 : 1));
-  const cudaError_t e = launch_attn<T, HDP, WM, true>(ctx, a, dim3(blocks));
+  const int blocks = min(kMaxBlocks, ctx->num_sms * (smem <= 100 * 1024 ? 2 : 1));
+  mdlc_note_launch(ctx);
+  e = launch_pdl(kern, dim3(blocks), dim3(kAttnThreads), smem, ctx->stream, a, ctx->d_err);
   if (e != cudaSuccess) return e;
   mdlc_note_launch(ctx);
   return launch_pdl(attn_join_kernel<T, HDP, WM>, dim3(a.d.kv_heads, a.d.batch), dim3(kJoinThreads), 0, ctx->stream, a, blocks);
 }
 
 template <typename T, int HDP>
-cudaError_t run_attn(mdlc_ctx* ctx, const AttnArgs& a) {
+cudaError_t run_attn(mdlc_ctx* ctx, AttnArgs& a) {
   const int wm = split_groups(a.d);
   cudaError_t e = cudaSuccess;
   if (wm == 1) e = run_split<T, HDP, 1>(ctx, a);
   else if (wm == 2) e = run_split<T, HDP, 2>(ctx, a);
   else if (wm == 4) e = run_split<T, HDP, 4>(ctx, a);
-  if (e != cudaSuccess || (long long)a.d.max_q * a.group <= a.split_rows) return e;
-  // row tiles at most: full ones, and one more per request
-  const int tiles = (int)((long long)a.d.tokens * a.group / Cfg<T, HDP, 4>::ROWS) + a.d.batch;
-  return launch_attn<T, HDP, 4, false>(ctx, a, dim3(tiles, a.d.kv_heads));
+  const Chunk c = chunk_of(a.d);
+  if (e != cudaSuccess || !c.used) return e;
+  a.splits = c.splits;
+  const dim3 grid(c.tiles, a.d.kv_heads, c.splits);
+  mdlc_note_launch(ctx);
+  if (c.tc) {
+    e = attn_tc_launch(ctx, a, grid);
+  } else {
+    const int smem = Cfg<T, HDP, 4>::SMEM;
+    e = cudaFuncSetAttribute(attn_chunk_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess) e = launch_pdl(attn_chunk_kernel<T, HDP>, grid, dim3(kAttnThreads), smem, ctx->stream, a, ctx->d_err);
+  }
+  if (e != cudaSuccess || c.splits == 1) return e;
+  mdlc_note_launch(ctx);
+  return launch_pdl(attn_chunk_join_kernel<T, HDP>, dim3(c.tiles, a.d.kv_heads, c.rows / 64), dim3(kJoinThreads), 0, ctx->stream, a, c.rows,
+                    c.tc ? kTcKeys : block_keys<T, HDP>());
 }
 
 }  // namespace

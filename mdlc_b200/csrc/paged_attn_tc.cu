@@ -1,0 +1,440 @@
+// Attention of chunks on tcgen05 (bf16): the products S = Q K^T and O = P V.
+//
+// A block takes 256 rows (two tiles of 128, one per softmax warpgroup) of one key head, so that
+// the 64 KB of keys and values of a 128-key block that it reads from L2 serve
+// 256 rows: 4 x 256 x 128 x d operations per 512 d bytes. Roles:
+//   warps 0-3, 4-7  softmax of row tile 0 / 1: a thread owns a row, reads its 128 scores from
+//                   tensor memory, keeps the running maximum and sum, writes the weights back
+//                   to tensor memory as bf16 (the A operand of the second product)
+//   warp 8          issues every MMA (one thread) and owns the tensor memory
+//   warp 9          loads keys and values by TMA, a box per page, 32 lanes at once
+// Tensor memory (512 columns): scores of the two tiles [0, 256), the weights over the first half of
+// their own tile's scores; outputs [256, 256 + 2 HDP). The MMA order per key block j is
+// O0 += P0(j) V(j), S0 = Q0 K(j+1), O1 += P1(j) V(j), S1 = Q1 K(j+1): while one tile's products run,
+// the other tile's weights are computed. Issue order makes S0(j+1) overwrite P0(j) only after it was read.
+// Outputs stay in tensor memory; they are rescaled only when a row's maximum grows by more than 2^8
+// over the one in use (weights are then at most 2^8; bf16 rounding is relative, so nothing is lost),
+// which after the first blocks hardly happens.
+// Keys past kv_len and pages that no row sees arrive as zeros: boxes out of the map's range, and the
+// last page's tail of the values is cleared in shared memory (its cache slots may hold NaN, and 0 x NaN
+// would reach every row).
+#include "conv.h"
+#include "paged_attn.cuh"
+
+namespace mdlc {
+namespace {
+
+constexpr int kThreads = 320;
+constexpr int kRows = kTcRows, kKeys = kTcKeys;
+constexpr int kRing = 4;             // key / value tiles in shared memory: K(j), V(j), K(j+1), V(j+1)
+constexpr float kGrow = 8.0f;        // growth of a row's maximum (base-2 exponent) that rescales the output
+constexpr unsigned long long kWaitCycles = 2 * kWaitLimitNs;
+
+template <int HDP>
+struct TcCfg {
+  static constexpr int HALVES = HDP / 64;               // 128-byte wide column blocks
+  static constexpr int TILE = 128 * HDP * 2;            // one Q tile, one key or value tile
+  static constexpr int Q = 0;
+  static constexpr int RING = 2 * TILE;
+  static constexpr int BARS = RING + kRing * TILE;
+  static constexpr int SMEM = BARS + 256 + 1024;        // 1024: alignment of the base
+  static constexpr int O_COL = 256;
+};
+// barriers
+enum { kFull = 0, kEmpty = kRing, kRaw = 2 * kRing, kQ, kS0, kS1, kP0, kP1, kO0, kO1, kDrain, kBars };
+
+// instruction descriptor: bf16 x bf16 -> fp32; B stored along its N axis (values)
+constexpr uint32_t idesc_bf16_nmajor(int M, int N) { return idesc_bf16(M, N) | (1u << 16); }
+
+// B operand stored along N: 64-column (128-byte) rows, one per k; 8-row groups 1024 bytes apart (SBO), the
+// next 64 columns lbo_bytes further
+MDLC_DEV uint64_t umma_desc_sw128_n(uint32_t saddr, uint32_t lbo_bytes) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo_bytes >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// A operand in tensor memory
+MDLC_DEV void umma_bf16_ta(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+#define MDLC_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+MDLC_DEV void tmem_ld32(uint32_t taddr, uint32_t* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,"
+      "%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : MDLC_R8(v, 0), MDLC_R8(v, 8), MDLC_R8(v, 16), MDLC_R8(v, 24)
+      : "r"(taddr)
+      : "memory");
+}
+MDLC_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int HDP>
+__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
+                                                              const __grid_constant__ CUtensorMap vmap, int* err) {
+  using C = TcCfg<HDP>;
+  extern __shared__ unsigned char tc_smem_raw[];
+  __shared__ long long warp_sums[kThreads / 32];
+  __shared__ Place place_s;
+  __shared__ uint32_t tmem_s;
+  __shared__ int abort_s;
+  unsigned char* smem = tc_smem_raw + ((1024 - (smem_u32(tc_smem_raw) & 1023)) & 1023);
+  const uint32_t sbase = smem_u32(smem);
+  auto bar = [&](int i) { return sbase + C::BARS + 8 * i; };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const mdlc_attn_desc& d = a.d;
+  volatile int* abort_flag = &abort_s;
+
+  if (warp == 9 && lane == 0) {
+    tma_prefetch_desc(&kmap);
+    tma_prefetch_desc(&vmap);
+  }
+  pdl_wait();
+  pdl_trigger();
+  Tile t;
+  if (!find_tile(a, blockIdx.x, kRows, warp_sums, &place_s, &t)) return;
+  const int e = blockIdx.y;
+  const Span sp = span_of(a, t.rq, t.r0 / a.group, (min(t.r0 + kRows, t.rows) - 1) / a.group, kKeys);
+  const int ns = splits_of(a, sp.n, 2);
+  if ((int)blockIdx.z >= ns) return;
+  const int blk0 = (int)((long long)blockIdx.z * sp.n / ns), blk1 = (int)((long long)(blockIdx.z + 1) * sp.n / ns), nb = blk1 - blk0;
+  const int shift = t.rq.kv_len - t.rq.q_len;
+  const int n_tiles = t.rows - t.r0 > 128 ? 2 : 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(bar(kFull + i), 1);
+      mbar_init(bar(kEmpty + i), 1);
+    }
+    mbar_init(bar(kRaw), 1);
+    mbar_init(bar(kQ), 256);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(kS0 + i), 1);
+      mbar_init(bar(kP0 + i), 128);
+      mbar_init(bar(kO0 + i), 1);
+    }
+    mbar_init(bar(kDrain), 1);
+    abort_s = 0;
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(&tmem_s), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ softmax
+    // queries: rows of 128 bytes per 64 columns, 16-byte chunks swizzled by the row
+    {
+      const int chunks = d.head_dim / 8;
+      constexpr int CH = HDP / 8;
+      for (int i = threadIdx.x; i < kRows * CH; i += 256) {
+        const int rl = i / CH, c = i % CH, r = t.r0 + rl;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < t.rows && c < chunks)
+          v = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + (long long)(t.rq.q0 + r / a.group) * d.q_stride +
+                                                   (long long)(e * a.group + r % a.group) * d.head_dim) + c);
+        *reinterpret_cast<uint4*>(smem + C::Q + (rl >> 7) * C::TILE + (c >> 3) * 16384 + (rl & 127) * 128 + (((c & 7) ^ (rl & 7)) << 4)) = v;
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(bar(kQ));
+    }
+    const int tile = warp >> 2, rl = threadIdx.x, r = t.r0 + rl;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_addr = tmem + lanes + tile * 128, o_addr = tmem + lanes + C::O_COL + tile * HDP;
+    const bool live = r < t.rows;
+    const int p = live ? shift + r / a.group : -1;
+    const int first = t.r0 + tile * 128, last = min(first + 127, t.rows - 1);
+    const int p_min = shift + first / a.group, p_max = shift + last / a.group;
+    const float c = a.scale_log2;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    if (tile < n_tiles) {
+      // page ids of a block, a lane each, to notice ids that do not exist (their keys are hidden)
+      const int box = min(d.page, kKeys), boxes = kKeys / box;
+      auto id_of = [&](int blk) {
+        int bad = 0;
+        if (lane < boxes && blk < blk1) {
+          const int j = key_of_block(sp, blk, kKeys) + lane * box;
+          if (j < sp.hi && (j + box > sp.lo || j < d.sinks))
+            bad = (unsigned)__ldg(a.table + (long long)t.b * d.table_stride + j / d.page) >= (unsigned)d.pages;
+        }
+        return bad;
+      };
+      int bad_next = id_of(blk0);
+      for (int j = 0; j < nb; ++j) {
+        const int base = key_of_block(sp, blk0 + j, kKeys);
+        const uint32_t bad = __ballot_sync(0xffffffffu, bad_next);
+        bad_next = id_of(blk0 + j + 1);
+        ok = mbar_wait(bar(kS0 + tile), j & 1, abort_flag, err, kWaitCycles);
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        // a block that every row of the tile sees whole needs no mask
+        const bool open = bad == 0 && base + kKeys - 1 <= p_min && (d.window == 0 || base > p_max - d.window || base + kKeys <= d.sinks);
+        const int hi = p - base, lo = d.window > 0 ? hi - d.window : -1, kept = d.window > 0 ? d.sinks - base : 0;
+        // 32 scores of the row, hidden keys at -inf
+        auto mask = [&](uint32_t (&s)[32], int k0) {
+          if (open) return;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const bool seen = k0 + i <= hi && (k0 + i > lo || k0 + i < kept);
+            s[i] = seen ? s[i] : 0xff800000u;
+          }
+          if (bad) {
+            const int lb = 31 - __clz(box);  // pages here are powers of two
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if ((bad >> ((k0 + i) >> lb)) & 1u) s[i] = 0xff800000u;
+          }
+        };
+        // the row is read twice, 32 scores at a time with the next 32 on their way: kept whole it would take
+        // 128 registers and spill
+        uint32_t s[2][32];
+        tmem_ld32(s_addr, s[0]);
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          tmem_ld_wait();
+          tmem_ld32(s_addr + 32 * ((k + 1) & 3), s[(k + 1) & 1]);
+          mask(s[k & 1], 32 * k);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[k & 1][i]));
+        }
+        const float mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        // a row that has summed nothing yet (its sum and output are zero) takes the maximum as it is
+        const bool fresh = m == -INFINITY, grow = !fresh && (mn - m) * c > kGrow;
+        const float f = grow ? ex2((m - mn) * c) : 1.0f;
+        if (fresh || grow) m = mn;
+        if (__any_sync(0xffffffffu, grow)) {
+          l *= f;
+          ok = mbar_wait(bar(kO0 + tile), (j - 1) & 1, abort_flag, err, kWaitCycles);
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < HDP; i += 16) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + i, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+            tmem_st16(o_addr + i, o);
+          }
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * c;
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          tmem_ld_wait();
+          if (k < 3) tmem_ld32(s_addr + 32 * (k + 1), s[(k + 1) & 1]);
+          mask(s[k & 1], 32 * k);
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float x = ex2(fmaf(__uint_as_float(s[k & 1][i]), c, -mc)), y = ex2(fmaf(__uint_as_float(s[k & 1][i + 1]), c, -mc));
+            sum[(i >> 1) & 3] += x + y;
+            w[i >> 1] = pack_bf16x2(x, y);
+          }
+          tmem_st16(s_addr + 16 * k, w);  // over scores that were read: columns 16 k .. 16 k + 15 of 32 k + 31
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(bar(kP0 + tile));
+      }
+      if (ok && nb > 0) ok = mbar_wait(bar(kO0 + tile), (nb - 1) & 1, abort_flag, err, kWaitCycles);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      if (ok) {
+        const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
+        const int tok = t.rq.q0 + r / a.group, head = e * a.group + r % a.group;
+        const long long slot = (((long long)blockIdx.x * d.kv_heads + e) * a.splits + blockIdx.z) * kRows + rl;
+        const float mlog = m == -INFINITY ? -INFINITY : m * c;
+        __nv_bfloat16* po = static_cast<__nv_bfloat16*>(a.out) + (long long)tok * d.out_stride + (long long)head * d.head_dim;
+        uint32_t o[HDP];
+#pragma unroll
+        for (int i = 0; i < HDP; ++i) o[i] = 0;
+        if (nb > 0) {
+#pragma unroll
+          for (int i = 0; i < HDP; i += 32) tmem_ld32(o_addr + i, o + i);
+          tmem_ld_wait();
+        }
+        if (live && ns == 1) {
+#pragma unroll
+          for (int k = 0; k < HDP; k += 8) {
+            if (k < d.head_dim) {
+              uint4 v;
+              v.x = pack_bf16x2(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
+              v.y = pack_bf16x2(__uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
+              v.z = pack_bf16x2(__uint_as_float(o[k + 4]) * inv, __uint_as_float(o[k + 5]) * inv);
+              v.w = pack_bf16x2(__uint_as_float(o[k + 6]) * inv, __uint_as_float(o[k + 7]) * inv);
+              *reinterpret_cast<uint4*>(po + k) = v;
+            }
+          }
+        } else if (live) {
+#pragma unroll
+          for (int k = 0; k < HDP; k += 4)
+            *reinterpret_cast<uint4*>(a.part_o + slot * HDP + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+        }
+        if (live) {
+          if (ns > 1) {
+            a.part_m[slot] = mlog;
+            a.part_l[slot] = l;
+          } else if (a.lse) {
+            a.lse[(long long)tok * d.heads + head] = (mlog + log2f(l)) * 0.69314718055994531f;
+          }
+        }
+      }
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ MMA
+    if (lane == 0 && nb > 0) {
+      constexpr uint32_t kIdS = idesc_bf16(128, kKeys), kIdO = idesc_bf16_nmajor(128, HDP);
+      bool ok = mbar_wait(bar(kQ), 0, abort_flag, err, kWaitCycles);
+      auto wait_tile = [&](int u) { return mbar_wait(bar(kFull + u % kRing), (u / kRing) & 1, abort_flag, err, kWaitCycles); };
+      auto scores = [&](int i, int j) {  // S_i = Q_i K(j)^T
+        const uint32_t q = sbase + C::Q + i * C::TILE, k = sbase + C::RING + ((2 * j) % kRing) * C::TILE;
+#pragma unroll
+        for (int ks = 0; ks < HDP / 16; ++ks) {
+          const uint32_t off = (ks / 4) * 16384 + (ks % 4) * 32;
+          umma_bf16(tmem + i * 128, umma_desc_sw128(q + off), umma_desc_sw128(k + off), kIdS, ks > 0);
+        }
+        umma_commit(bar(kS0 + i));
+      };
+      ok = ok && wait_tile(0);
+      tc_fence_after();
+      if (ok) {
+        for (int i = 0; i < n_tiles; ++i) scores(i, 0);
+        umma_commit(bar(kEmpty + 0));
+      }
+      for (int j = 0; ok && j < nb; ++j) {
+        ok = wait_tile(2 * j + 1);
+        for (int i = 0; ok && i < n_tiles; ++i) {
+          ok = mbar_wait(bar(kP0 + i), j & 1, abort_flag, err, kWaitCycles);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t v = sbase + C::RING + ((2 * j + 1) % kRing) * C::TILE;
+#pragma unroll
+          for (int ks = 0; ks < kKeys / 16; ++ks)
+            umma_bf16_ta(tmem + C::O_COL + i * HDP, tmem + i * 128 + ks * 8, umma_desc_sw128_n(v + ks * 2048, 16384), kIdO, j > 0 || ks > 0);
+          umma_commit(bar(kO0 + i));
+          if (i == n_tiles - 1) umma_commit(bar(kEmpty + (2 * j + 1) % kRing));
+          if (j + 1 < nb) {
+            if (i == 0) {
+              ok = wait_tile(2 * j + 2);
+              if (!ok) break;
+              tc_fence_after();
+            }
+            scores(i, j + 1);
+            if (i == n_tiles - 1) umma_commit(bar(kEmpty + (2 * j + 2) % kRing));
+          }
+        }
+      }
+      // everything issued is done before the tensor memory goes back
+      umma_commit(bar(kDrain));
+      mbar_wait(bar(kDrain), 0, nullptr, err, kWaitCycles);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ keys and values
+    const int box = min(d.page, kKeys), boxes = kKeys / box;
+    const int page_i = lane % boxes, half = lane / boxes;   // this lane's box: boxes x HALVES <= 32 of them
+    const bool mine = half < C::HALVES;
+    const int none = d.pages * d.kv_heads * d.page;         // a row past the map: zeros
+    bool ok = true;
+    int u = 0, raw = 0;
+    for (int j = 0; ok && j < nb; ++j) {
+      const int base = key_of_block(sp, blk0 + j, kKeys);
+      const int k0 = base + page_i * box;
+      int row = none;
+      if (mine && k0 < sp.hi && (k0 + box > sp.lo || k0 < d.sinks)) {
+        const int id = __ldg(a.table + (long long)t.b * d.table_stride + k0 / d.page);
+        if ((unsigned)id < (unsigned)d.pages) row = (id * d.kv_heads + e) * d.page + k0 % d.page;
+        else record_error(err, MDLC_DEVERR_BOUNDS);
+      }
+      for (int kv = 0; kv < 2; ++kv, ++u) {
+        const int st = u % kRing;
+        // values whose last page ends inside this block: cleared from kv_len on before the MMA may read them
+        const bool tail = kv == 1 && base < t.rq.kv_len && t.rq.kv_len < base + kKeys && t.rq.kv_len % d.page != 0;
+        if (u >= kRing) ok = mbar_wait(bar(kEmpty + st), ((u / kRing) & 1) ^ 1, abort_flag, err, kWaitCycles);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t full = tail ? bar(kRaw) : bar(kFull + st);
+        if (lane == 0) mbar_arrive_expect_tx(full, C::TILE);
+        __syncwarp();
+        const uint32_t dst = sbase + C::RING + st * C::TILE;
+        if (mine) tma_load_2d(dst + half * 16384 + page_i * box * 128, kv ? &vmap : &kmap, half * 64, row, full);
+        if (tail) {
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(kRaw), raw & 1, nullptr, err, kWaitCycles));
+          ++raw;
+          if (!ok) break;
+          const int z0 = t.rq.kv_len - base, z1 = min(kKeys, (z0 / box + 1) * box);
+          for (int i = lane; i < (z1 - z0) * 8 * C::HALVES; i += 32) {
+            const int h = i / ((z1 - z0) * 8), k = i % ((z1 - z0) * 8);
+            *reinterpret_cast<uint4*>(smem + C::RING + st * C::TILE + h * 16384 + (z0 + k / 8) * 128 + (k % 8) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(kFull + st));
+        }
+      }
+    }
+    if (!ok) {
+      // given up: this block's copies must land before its shared memory goes back
+      for (int i = max(0, u - kRing); i < u; ++i) mbar_wait(bar(kFull + i % kRing), (i / kRing) & 1, nullptr, err, kWaitCycles);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 8) tmem_dealloc(tmem, 512);
+}
+
+template <int HDP>
+cudaError_t launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid) {
+  const auto encode = tensor_map_encoder();
+  if (!encode) return cudaErrorNotSupported;
+  const mdlc_attn_desc& d = a.d;
+  // a cache as rows of head_dim elements, one per (page, key head, token)
+  const cuuint64_t dims[2] = {(cuuint64_t)d.head_dim, (cuuint64_t)d.pages * d.kv_heads * d.page};
+  const cuuint64_t strides[1] = {(cuuint64_t)d.head_dim * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)min(d.page, kKeys)}, steps[2] = {1, 1};
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i)
+    if (encode(&maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(i ? a.v : a.k), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return cudaErrorInvalidValue;
+  const cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel<HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<HDP>::SMEM);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(attn_tc_kernel<HDP>, grid, dim3(kThreads), TcCfg<HDP>::SMEM, ctx->stream, a, maps[0], maps[1], ctx->d_err);
+}
+
+}  // namespace
+
+// bf16, pages that tile a 128-key block, a positive scale (the running maximum is that of the raw scores)
+bool attn_tc_fits(const mdlc_attn_desc& d) {
+  const bool page = d.page >= 8 && (d.page & (d.page - 1)) == 0;
+  return d.dtype == MDLC_BF16 && page && d.scale > 0.0f;
+}
+
+cudaError_t attn_tc_launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid) {
+  return a.d.head_dim <= 64 ? launch<64>(ctx, a, grid) : launch<128>(ctx, a, grid);
+}
+
+}  // namespace mdlc
