@@ -582,7 +582,7 @@ Chunk chunk_of(const mdlc_attn_desc& d) {
   const int group = d.heads / d.kv_heads;
   Chunk c = {};
   c.used = (long long)d.max_q * group > 16 * split_groups(d);
-  c.tc = attn_tc_fits(d);
+  c.tc = attn_tc_fits(d) && (long long)d.tokens * group / kTcRows + d.batch <= 65535;  // the tiles are its grid's y
   c.rows = c.tc ? kTcRows : 64;
   c.tiles = (int)min((long long)d.tokens * group / c.rows + d.batch, (long long)INT32_MAX);
   // the mma.sync kernel runs three blocks per SM

@@ -8,6 +8,7 @@
 //                   to tensor memory as bf16 (the A operand of the second product)
 //   warp 8          issues every MMA (one thread) and owns the tensor memory
 //   warp 9          loads keys and values by TMA, a box per page, 32 lanes at once
+//   (warps 8-11 give registers to the softmax warpgroups; 10 and 11 do nothing else)
 // Tensor memory (512 columns): scores of the two tiles [0, 256), the weights over the first half of
 // their own tile's scores; outputs [256, 256 + 2 HDP). The MMA order per key block j is
 // O0 += P0(j) V(j), S0 = Q0 K(j+1), O1 += P1(j) V(j), S1 = Q1 K(j+1): while one tile's products run,
@@ -24,7 +25,9 @@
 namespace mdlc {
 namespace {
 
-constexpr int kThreads = 320;
+constexpr int kThreads = 384;
+// registers of a softmax and of another thread: 2 x 128 x 208 + 128 x 88 = 384 x 168, what the block is launched with
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 constexpr int kRows = kTcRows, kKeys = kTcKeys;
 constexpr int kRing = 4;             // key / value tiles in shared memory: K(j), V(j), K(j+1), V(j+1)
 constexpr float kGrow = 8.0f;        // growth of a row's maximum (base-2 exponent) that rescales the output
@@ -69,6 +72,28 @@ MDLC_DEV void tmem_ld32(uint32_t taddr, uint32_t* v) {
       : "r"(taddr)
       : "memory");
 }
+#define MDLC_I8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+MDLC_DEV void tmem_st32(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      MDLC_I8(v, 0), MDLC_I8(v, 8), MDLC_I8(v, 16), MDLC_I8(v, 24)
+      : "memory");
+}
+MDLC_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+MDLC_DEV float2 add2(const float2 a, const float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_from(r);
+}
+template <int N>
+MDLC_DEV void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+MDLC_DEV void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 MDLC_DEV float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -98,8 +123,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
   pdl_wait();
   pdl_trigger();
   Tile t;
-  if (!find_tile(a, blockIdx.x, kRows, warp_sums, &place_s, &t)) return;
-  const int e = blockIdx.y;
+  if (!find_tile(a, blockIdx.y, kRows, warp_sums, &place_s, &t)) return;
+  const int e = blockIdx.x;
   const Span sp = span_of(a, t.rq, t.r0 / a.group, (min(t.r0 + kRows, t.rows) - 1) / a.group, kKeys);
   const int ns = splits_of(a, sp.n, 2);
   if ((int)blockIdx.z >= ns) return;
@@ -134,6 +159,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax
+    regs_up<kSoftmaxRegs>();
     // queries: rows of 128 bytes per 64 columns, 16-byte chunks swizzled by the row
     {
       const int chunks = d.head_dim / 8;
@@ -161,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
     bool ok = true;
     if (tile < n_tiles) {
       // page ids of a block, a lane each, to notice ids that do not exist (their keys are hidden)
-      const int box = min(d.page, kKeys), boxes = kKeys / box;
+      const int box = min(d.page, kKeys), boxes = kKeys / box, box_log2 = 31 - __clz(box);  // a power of two
       auto id_of = [&](int blk) {
         int bad = 0;
         if (lane < boxes && blk < blk1) {
@@ -185,74 +211,76 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
         // a block that every row of the tile sees whole needs no mask
         const bool open = bad == 0 && base + kKeys - 1 <= p_min && (d.window == 0 || base > p_max - d.window || base + kKeys <= d.sinks);
         const int hi = p - base, lo = d.window > 0 ? hi - d.window : -1, kept = d.window > 0 ? d.sinks - base : 0;
-        // 32 scores of the row, hidden keys at -inf
-        auto mask = [&](uint32_t (&s)[32], int k0) {
-          if (open) return;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const bool seen = k0 + i <= hi && (k0 + i > lo || k0 + i < kept);
-            s[i] = seen ? s[i] : 0xff800000u;
-          }
-          if (bad) {
-            const int lb = 31 - __clz(box);  // pages here are powers of two
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if ((bad >> ((k0 + i) >> lb)) & 1u) s[i] = 0xff800000u;
-          }
-        };
-        // the row is read twice, 32 scores at a time with the next 32 on their way: kept whole it would take
-        // 128 registers and spill
-        uint32_t s[2][32];
-        tmem_ld32(s_addr, s[0]);
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          tmem_ld_wait();
-          tmem_ld32(s_addr + 32 * ((k + 1) & 3), s[(k + 1) & 1]);
-          mask(s[k & 1], 32 * k);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(s[k & 1][i]));
-        }
-        const float mn = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        // a row that has summed nothing yet (its sum and output are zero) takes the maximum as it is
-        const bool fresh = m == -INFINITY, grow = !fresh && (mn - m) * c > kGrow;
-        const float f = grow ? ex2((m - mn) * c) : 1.0f;
-        if (fresh || grow) m = mn;
-        if (__any_sync(0xffffffffu, grow)) {
-          l *= f;
-          ok = mbar_wait(bar(kO0 + tile), (j - 1) & 1, abort_flag, err, kWaitCycles);
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-#pragma unroll
-          for (int i = 0; i < HDP; i += 16) {
-            uint32_t o[16];
-            tmem_ld16(o_addr + i, o);
+        if (!open) {
+          // hidden keys to -inf, in place (a loop of its own, so that the common path stays small)
+#pragma unroll 1
+          for (int k0 = 0; k0 < kKeys; k0 += 32) {
+            uint32_t s[32];
+            tmem_ld32(s_addr + k0, s);
             tmem_ld_wait();
 #pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-            tmem_st16(o_addr + i, o);
+            for (int i = 0; i < 32; ++i) {
+              const bool seen = k0 + i <= hi && (k0 + i > lo || k0 + i < kept) && !((bad >> ((k0 + i) >> box_log2)) & 1u);
+              s[i] = seen ? s[i] : 0xff800000u;
+            }
+            tmem_st32(s_addr + k0, s);
+          }
+          tmem_st_wait();
+        }
+        // One pass takes the weights against the maximum in use and the block's own maximum; when that has grown
+        // by more than 2^8 for some row of the warp (or a row sees its first keys) the pass is
+        // repeated with the new one. The weights wait in registers: their place is the scores' own.
+        uint32_t w[64];
+        for (;;) {
+          const float mc = m == -INFINITY ? 0.0f : m * c;
+          const float2 c2 = splat2(c), mc2 = splat2(-mc);
+          float top[2] = {-INFINITY, -INFINITY};
+          float2 sum[2] = {splat2(0.0f), splat2(0.0f)};
+          uint32_t s[2][32];
+          tmem_ld32(s_addr, s[0]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            tmem_ld_wait();
+            if (k < 3) tmem_ld32(s_addr + 32 * (k + 1), s[(k + 1) & 1]);
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 x = make_float2(__uint_as_float(s[k & 1][i]), __uint_as_float(s[k & 1][i + 1]));
+              top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], x.x, x.y);
+              float2 y = fma2(x, c2, mc2);
+              y = make_float2(ex2(y.x), ex2(y.y));
+              sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], y);
+              w[16 * k + (i >> 1)] = pack_bf16x2(y.x, y.y);
+            }
+          }
+          const float mn = fmaxf(top[0], top[1]);
+          const bool fresh = m == -INFINITY && mn > -INFINITY, grow = m != -INFINITY && (mn - m) * c > kGrow;
+          if (!__any_sync(0xffffffffu, fresh || grow)) {
+            l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+            break;
+          }
+          // a row that has summed nothing yet (sum and output are zero) takes the maximum as it is
+          const float f = grow ? ex2((m - mn) * c) : 1.0f;
+          if (fresh || grow) m = mn;
+          if (__any_sync(0xffffffffu, grow)) {
+            l *= f;
+            ok = mbar_wait(bar(kO0 + tile), (j - 1) & 1, abort_flag, err, kWaitCycles);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int i = 0; i < HDP; i += 32) {
+              uint32_t o[32];
+              tmem_ld32(o_addr + i, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+              tmem_st32(o_addr + i, o);
+            }
           }
         }
-        const float mc = m == -INFINITY ? 0.0f : m * c;
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          tmem_ld_wait();
-          if (k < 3) tmem_ld32(s_addr + 32 * (k + 1), s[(k + 1) & 1]);
-          mask(s[k & 1], 32 * k);
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float x = ex2(fmaf(__uint_as_float(s[k & 1][i]), c, -mc)), y = ex2(fmaf(__uint_as_float(s[k & 1][i + 1]), c, -mc));
-            sum[(i >> 1) & 3] += x + y;
-            w[i >> 1] = pack_bf16x2(x, y);
-          }
-          tmem_st16(s_addr + 16 * k, w);  // over scores that were read: columns 16 k .. 16 k + 15 of 32 k + 31
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (!ok) break;
+        tmem_st32(s_addr, w);
+        tmem_st32(s_addr + 32, w + 32);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(bar(kP0 + tile));
@@ -263,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
       if (ok) {
         const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
         const int tok = t.rq.q0 + r / a.group, head = e * a.group + r % a.group;
-        const long long slot = (((long long)blockIdx.x * d.kv_heads + e) * a.splits + blockIdx.z) * kRows + rl;
+        const long long slot = (((long long)blockIdx.y * d.kv_heads + e) * a.splits + blockIdx.z) * kRows + rl;
         const float mlog = m == -INFINITY ? -INFINITY : m * c;
         __nv_bfloat16* po = static_cast<__nv_bfloat16*>(a.out) + (long long)tok * d.out_stride + (long long)head * d.head_dim;
         uint32_t o[HDP];
@@ -301,7 +329,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
         }
       }
     }
-  } else if (warp == 8) {
+  } else {
+    regs_down<kOtherRegs>();  // warps 8 to 11 alike, before their ways part
+    if (warp == 8) {
     // ------------------------------------------------------------ MMA
     if (lane == 0 && nb > 0) {
       constexpr uint32_t kIdS = idesc_bf16(128, kKeys), kIdO = idesc_bf16_nmajor(128, HDP);
@@ -350,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
       mbar_wait(bar(kDrain), 0, nullptr, err, kWaitCycles);
     }
     __syncwarp();
-  } else {
+    } else if (warp == 9) {
     // ------------------------------------------------------------ keys and values
     const int box = min(d.page, kKeys), boxes = kKeys / box;
     const int page_i = lane % boxes, half = lane / boxes;   // this lane's box: boxes x HALVES <= 32 of them
@@ -398,6 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
       // given up: this block's copies must land before its shared memory goes back
       for (int i = max(0, u - kRing); i < u; ++i) mbar_wait(bar(kFull + i % kRing), (i / kRing) & 1, nullptr, err, kWaitCycles);
     }
+    }
   }
   __syncwarp();
   tc_fence_before();
@@ -422,7 +453,8 @@ cudaError_t launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid) {
       return cudaErrorInvalidValue;
   const cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel<HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<HDP>::SMEM);
   if (e != cudaSuccess) return e;
-  return launch_pdl(attn_tc_kernel<HDP>, grid, dim3(kThreads), TcCfg<HDP>::SMEM, ctx->stream, a, maps[0], maps[1], ctx->d_err);
+  // key heads fastest: the tiles that see the most keys start first in all of them
+  return launch_pdl(attn_tc_kernel<HDP>, dim3(grid.y, grid.x, grid.z), dim3(kThreads), TcCfg<HDP>::SMEM, ctx->stream, a, maps[0], maps[1], ctx->d_err);
 }
 
 }  // namespace
