@@ -14,8 +14,9 @@
 //   split mode (few rows per request: decoding): bounded by the cache's bytes. The
 //     keys of all (request, key head) tiles form one line of 128-key units, cut evenly
 //     over the blocks whatever the requests' lengths; a tile cut between blocks leaves
-//     partial sums in the workspace, which attn_join_kernel adds in block order.
-//   chunk mode (many rows): a block per row tile.
+//     partial sums in the workspace, which the last of them to arrive adds in block order.
+//   chunk mode (many rows): a block per row tile, or several that share its keys.
+#include "func_attr.h"
 #include "paged_attn.cuh"
 
 namespace mdlc {
@@ -359,37 +360,101 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
 // the block that holds unit u when `units` are cut into `blocks` runs [c units / blocks, (c + 1) units / blocks)
 MDLC_DEV int block_of(long long u, long long units, int blocks) { return (int)(((u + 1) * blocks - 1) / units); }
 
-template <typename T, int HDP, int WM>
-__global__ void __launch_bounds__(kAttnThreads) attn_split_kernel(const AttnArgs a, int* err) {
-  using K = Cfg<T, HDP, WM>;
-  constexpr int UB = kUnit / K::BT;
-  extern __shared__ __align__(128) unsigned char attn_smem[];
-  __shared__ uint32_t valid_s[K::WN][kStages];
+// Split mode: a piece of a tile that blocks c0 .. c1 share is in the workspace. The last of them to arrive adds all
+// pieces, in block order whoever it is, so the result does not depend on timing.
+template <typename T, int HDP, int ROWS>
+MDLC_DEV void join_pieces(const AttnArgs& a, int b, int e, const Request& rq, int c0, int c1) {
+  constexpr int V = HDP / 32, NW = kAttnThreads / 32;
+  __shared__ float part[NW][HDP + 2];
+  __shared__ int last_s;
+  const mdlc_attn_desc& d = a.d;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    last_s = atomicAdd(a.arrived + c0, 1) == c1 - c0;
+    if (last_s) a.arrived[c0] = 0;
+  }
+  __syncthreads();
+  if (!last_s) return;
+  __threadfence();
+  const int rows = rq.q_len * a.group;
+  const long long slot0 = (long long)b * d.kv_heads + e;
+  int wpr = 1;  // warps of a row, each with every wpr-th piece
+  while (wpr * 2 * rows <= NW) wpr *= 2;
+  const int rpb = NW / wpr;
+  for (int rb = 0; rb < rows; rb += rpb) {
+    const int r = rb + warp / wpr, w = warp % wpr;
+    float top = -INFINITY, sum = 0.0f, acc[V] = {};
+    if (r < rows) {
+#pragma unroll 4
+      for (int c = c0 + w; c <= c1; c += wpr) {
+        const long long at = (slot0 + c) * ROWS + r;
+        const float pm = __ldcg(a.part_m + at), pl = __ldcg(a.part_l + at);
+        float x[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] = __ldcg(a.part_o + at * HDP + i * 32 + lane);
+        const float mn = fmaxf(top, pm), safe = mn == -INFINITY ? 0.0f : mn;
+        const float f0 = exp2f(top - safe), f1 = exp2f(pm - safe);
+        top = mn;
+        sum = sum * f0 + pl * f1;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = acc[i] * f0 + x[i] * f1;
+      }
+    }
+    if (wpr > 1) {
+      __syncthreads();
+      if (lane == 0) {
+        part[warp][HDP] = top;
+        part[warp][HDP + 1] = sum;
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) part[warp][i * 32 + lane] = acc[i];
+      __syncthreads();
+      if (w == 0) {
+        for (int k = 1; k < wpr; ++k) {
+          const float pm = part[warp + k][HDP], mn = fmaxf(top, pm), safe = mn == -INFINITY ? 0.0f : mn;
+          const float f0 = exp2f(top - safe), f1 = exp2f(pm - safe);
+          top = mn;
+          sum = sum * f0 + part[warp + k][HDP + 1] * f1;
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[i] = acc[i] * f0 + part[warp + k][i * 32 + lane] * f1;
+        }
+      }
+    }
+    if (w == 0 && r < rows) {
+      const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+      const int tok = rq.q0 + r / a.group, head = e * a.group + r % a.group;
+      T* po = static_cast<T*>(a.out) + (long long)tok * d.out_stride + (long long)head * d.head_dim;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i * 32 + lane < d.head_dim) store_out<T>(po + i * 32 + lane, acc[i] * inv);
+      if (a.lse && lane == 0) a.lse[(long long)tok * d.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
+    }
+  }
+  __syncthreads();
+}
+
+// Split mode's line of work: calls piece(b, request, e, span, first block, end, whole, slot) for every run of this
+// block's units that lies in one tile, and join(b, request, e, c0, c1) after a piece of a shared tile.
+template <int BT, typename Piece, typename Join>
+MDLC_DEV void split_walk(const AttnArgs& a, Piece piece, Join join) {
+  constexpr int UB = kUnit / BT;
   __shared__ long long warp_sums[kAttnThreads / 32];
   __shared__ Place place_s;
-  pdl_wait();
-  pdl_trigger();
   const mdlc_attn_desc& d = a.d;
   // units of a request and key head
   auto units_of = [&](int b) -> long long {
     const Request r = request_of(a, b);
     const long long rows = (long long)r.q_len * a.group;
     if (rows == 0 || rows > a.split_rows) return 0;
-    return max(1, (span_of(a, r, 0, r.q_len - 1, K::BT).n + UB - 1) / UB);
+    return max(1, (span_of(a, r, 0, r.q_len - 1, BT).n + UB - 1) / UB);
   };
   const int per = (d.batch + kAttnThreads - 1) / kAttnThreads;
   const int b0 = min((int)threadIdx.x * per, d.batch), b1 = min(b0 + per, d.batch);
   long long mine = 0, total;
   for (int b = b0; b < b1; ++b) mine += units_of(b) * d.kv_heads;
   const long long before = block_scan(mine, warp_sums, &total);
-  if (blockIdx.x == 0) {
-    long long at = before;
-    for (int b = b0; b < b1; ++b) {
-      a.first_unit[b] = at;
-      at += units_of(b) * d.kv_heads;
-      if (b == d.batch - 1) a.first_unit[d.batch] = at;
-    }
-  }
   const int blocks = (int)min((long long)gridDim.x, total);
   if ((int)blockIdx.x >= blocks) return;
   long long u0 = (long long)blockIdx.x * total / blocks;
@@ -417,12 +482,308 @@ __global__ void __launch_bounds__(kAttnThreads) attn_split_kernel(const AttnArgs
     }
     const int e = (int)((u0 - pl.first) / n);
     const long long tile0 = pl.first + e * n, end = min(u1, tile0 + n);
-    const Span sp = span_of(a, rq, 0, rq.q_len - 1, K::BT);
+    const Span sp = span_of(a, rq, 0, rq.q_len - 1, BT);
     const int blk0 = (int)(u0 - tile0) * UB, blk1 = min((int)(end - tile0) * UB, sp.n);
-    attn_piece<T, HDP, WM>(a, attn_smem, valid_s, err, pl.b, rq, e, 0, sp, blk0, blk1, u0 == tile0 && end == tile0 + n,
-                           (long long)pl.b * d.kv_heads + e + blockIdx.x);
+    const bool whole = u0 == tile0 && end == tile0 + n;
+    piece(pl.b, rq, e, sp, blk0, blk1, whole, (long long)pl.b * d.kv_heads + e + blockIdx.x);
+    if (!whole) join(pl.b, rq, e, block_of(tile0, total, blocks), block_of(tile0 + n - 1, total, blocks));
     u0 = end;
   }
+}
+
+template <typename T, int HDP, int WM>
+__global__ void __launch_bounds__(kAttnThreads) attn_split_kernel(const AttnArgs a, int* err) {
+  using K = Cfg<T, HDP, WM>;
+  extern __shared__ __align__(128) unsigned char attn_smem[];
+  __shared__ uint32_t valid_s[K::WN][kStages];
+  pdl_wait();
+  pdl_trigger();
+  split_walk<K::BT>(
+      a,
+      [&](int b, const Request& rq, int e, const Span& sp, int blk0, int blk1, bool whole, long long slot) {
+        attn_piece<T, HDP, WM>(a, attn_smem, valid_s, err, b, rq, e, 0, sp, blk0, blk1, whole, slot);
+      },
+      [&](int b, const Request& rq, int e, int c0, int c1) { join_pieces<T, HDP, K::ROWS>(a, b, e, rq, c0, c1); });
+}
+
+// ------------------------------------------------------------ few rows, bf16
+// Decoding in bf16 with at most 16 rows per tile and pages of 8, 16, 32, ... keys: the same split mode with the roles of the
+// operands turned. The 16 rows of a product are keys (S^T = K Q^T) or output columns (O^T = V^T P^T) and the 8 columns are
+// the tile's rows, so that 8 rows cost half the products, registers and exponentials that 16 would; the weights go
+// from the first product's result to the second one's operand through movmatrix, the 8 x 8 transpose.
+// Every warp has its own ring of 32-key blocks, filled by TMA (a box per page and 64 columns, issued
+// by as many lanes). Bounded by the cache's bytes: NARROW_FIGURES.
+template <int HDP, int NT>
+struct NarrowCfg {
+  static constexpr int BT = 32, ROWS = 16;                 // workspace slots hold 16 rows
+  static constexpr int TILE = BT * HDP * 2;                // keys or values of a block
+  static constexpr int STAGES = 3;
+  static constexpr int RING = 4 * STAGES * 2 * TILE;
+  static constexpr int OP = HDP + 4;                       // floats of a row of the merge
+  static constexpr int SMEM = RING + 1024;                 // 1024: alignment
+};
+MDLC_DEV uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+MDLC_DEV float max_over_keys(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+}
+MDLC_DEV float sum_over_keys(float v) {
+  v += __shfl_xor_sync(0xffffffffu, v, 4);
+  v += __shfl_xor_sync(0xffffffffu, v, 8);
+  return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+
+template <int HDP, int NT>
+__global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
+                                                                      const __grid_constant__ CUtensorMap vmap, int* err) {
+  using C = NarrowCfg<HDP, NT>;
+  constexpr int BT = C::BT, HALVES = HDP / 64, MT = HDP / 16;
+  extern __shared__ unsigned char narrow_raw[];
+  __shared__ __align__(8) uint64_t full_s[4][C::STAGES];
+  unsigned char* smem = narrow_raw + ((1024 - (smem_u32(narrow_raw) & 1023)) & 1023);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const mdlc_attn_desc& d = a.d;
+  if (threadIdx.x < 4 * C::STAGES) mbar_init(smem_u32(&full_s[0][0] + threadIdx.x), 1);
+  fence_mbar_init();
+  if (lane == 0) {
+    tma_prefetch_desc(&kmap);
+    tma_prefetch_desc(&vmap);
+  }
+  pdl_wait();
+  pdl_trigger();
+  const uint32_t ring = smem_u32(smem) + warp * C::STAGES * 2 * C::TILE;
+  unsigned char* ring_p = smem + warp * C::STAGES * 2 * C::TILE;
+  const int box = min(d.page, BT), boxes = BT / box;       // keys of a TMA box, boxes of a block
+  const int none = d.pages * d.kv_heads * d.page;          // a row past the maps: zeros
+  // this lane's box: keys or values, 64-column half, page
+  const int my_page = lane % boxes, my_half = lane / boxes % HALVES, my_kv = lane / (boxes * HALVES);
+  const bool mine = my_kv < 2;
+  uint32_t begun = 0, used = 0;  // blocks issued and consumed by this warp so far
+
+  auto piece = [&](int b, const Request& rq, int e, const Span& sp, int blk0, int blk1, bool whole, long long slot) {
+    const int rows = rq.q_len * a.group, shift = rq.kv_len - rq.q_len;
+    // queries as the column operand: row 8 n + g, columns 16 ks + 2 t and + 8
+    uint32_t qb[MT][NT][2];
+    int pos[NT][2];  // positions of this thread's result columns, rows 8 n + 2 t and + 1
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = 8 * n + g;
+      const __nv_bfloat16* qp = static_cast<const __nv_bfloat16*>(a.q) + (long long)(rq.q0 + min(r, rows - 1) / a.group) * d.q_stride +
+                                (long long)(e * a.group + min(r, rows - 1) % a.group) * d.head_dim;
+#pragma unroll
+      for (int ks = 0; ks < MT; ++ks)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = 16 * ks + 2 * t + 8 * i;
+          qb[ks][n][i] = (r < rows && c < d.head_dim) ? __ldg(reinterpret_cast<const uint32_t*>(qp + c)) : 0u;
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) pos[n][i] = 8 * n + 2 * t + i < rows ? shift + (8 * n + 2 * t + i) / a.group : -1;
+    }
+    // cache row of this lane's box (a row past the maps: hidden or missing), and whether its page exists
+    auto row_of = [&](int blk) {
+      if (blk >= blk1 || !mine) return none;
+      const int k0 = key_of_block(sp, blk, BT) + my_page * box;
+      if (k0 >= sp.hi || (k0 + box <= sp.lo && k0 >= d.sinks)) return none;
+      const int id = __ldg(a.table + (long long)b * d.table_stride + k0 / d.page);
+      if ((unsigned)id < (unsigned)d.pages) return (id * d.kv_heads + e) * d.page + k0 % d.page;
+      record_error(err, MDLC_DEVERR_BOUNDS);
+      return none;
+    };
+    uint32_t there[C::STAGES];  // bit p: box p of the block in that stage was loaded
+    auto issue = [&](int blk, int row, int st) {
+      const uint32_t have = __ballot_sync(0xffffffffu, row != none);
+#pragma unroll
+      for (int i = 0; i < C::STAGES; ++i)
+        if (i == st) there[i] = have & ((1u << boxes) - 1u);
+      if (blk >= blk1) return;
+      const uint32_t bar = smem_u32(&full_s[warp][st]);
+      if (lane == 0) mbar_arrive_expect_tx(bar, 2 * C::TILE);
+      __syncwarp();
+      if (mine)
+        tma_load_2d(ring + st * 2 * C::TILE + my_kv * C::TILE + my_half * (BT * 128) + my_page * box * 128, my_kv ? &vmap : &kmap, my_half * 64, row, bar);
+      ++begun;
+    };
+    float o[MT][NT][4] = {};
+    float m[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) m[n][0] = m[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.0f;
+    // this warp takes blocks blk0 + warp, blk0 + warp + 4, ...; the stage of a use is its number modulo STAGES
+    int st = used % C::STAGES;
+    auto next_stage = [&](int s, int by) { return (s + by) % C::STAGES; };
+    for (int i = 0; i < C::STAGES - 1; ++i) issue(blk0 + warp + 4 * i, row_of(blk0 + warp + 4 * i), next_stage(st, i));
+    int row_next = row_of(blk0 + warp + 4 * (C::STAGES - 1));
+    bool ok = true;
+    for (int blk = blk0 + warp; blk < blk1; blk += 4) {
+      __syncwarp();  // every lane has read the stage that is filled next
+      issue(blk + 4 * (C::STAGES - 1), row_next, next_stage(st, C::STAGES - 1));
+      row_next = row_of(blk + 4 * C::STAGES);
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_s[warp][st]), (used / C::STAGES) & 1, nullptr, err, 2 * kWaitLimitNs));
+      if (!ok) break;
+      ++used;
+      const uint32_t ks_addr = ring + st * 2 * C::TILE, vs_addr = ks_addr + C::TILE;
+      const int base = key_of_block(sp, blk, BT);
+      uint32_t have = 0;
+#pragma unroll
+      for (int i = 0; i < C::STAGES; ++i)
+        if (i == st) have = there[i];
+      if (base + BT > rq.kv_len && base < rq.kv_len) {
+        // values past kv_len may be anything (0 x NaN): cleared
+        const int z0 = rq.kv_len - base;
+        for (int i = lane; i < (BT - z0) * 8 * HALVES; i += 32) {
+          const int h = i / ((BT - z0) * 8), k = i % ((BT - z0) * 8);
+          *reinterpret_cast<uint4*>(ring_p + st * 2 * C::TILE + C::TILE + h * (BT * 128) + (z0 + k / 8) * 128 + (k % 8) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      // scores: 16-key tile mt, rows 8 n + 2 t
+      float s[2][NT][4] = {};
+      {
+        const int mi = lane >> 3, r = lane & 7, key = (mi & 1) * 8 + r;
+#pragma unroll
+        for (int ks = 0; ks < MT; ++ks)
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+            uint32_t ka[4];
+            const int ch = 2 * ks + (mi >> 1);
+            ldsm_x4(ka, ks_addr + (ch >> 3) * (BT * 128) + (mt * 16 + key) * 128 + (((ch & 7) ^ r) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_bf16(s[mt][n], ka, qb[ks][n][0], qb[ks][n][1]);
+          }
+      }
+      const bool open = have == (1u << boxes) - 1u && base + BT - 1 <= shift &&
+                        (d.window == 0 || base > shift + rq.q_len - 1 - d.window || base + BT <= d.sinks);
+      bool grew = false;
+      float safe[NT][2], shrink[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float top = -INFINITY;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float x = s[mt][n][2 * h + i] * a.scale_log2;
+              if (!open) {
+                const int c = mt * 16 + h * 8 + g, j = base + c, p = pos[n][i];
+                const bool seen = ((have >> (c / box)) & 1u) && j <= p && (d.window == 0 || j > p - d.window || j < d.sinks);
+                x = seen ? x : -INFINITY;
+              }
+              s[mt][n][2 * h + i] = x;
+              top = fmaxf(top, x);
+            }
+          const float mn = fmaxf(m[n][i], max_over_keys(top));
+          safe[n][i] = mn == -INFINITY ? 0.0f : mn;
+          shrink[n][i] = exp2f(m[n][i] - safe[n][i]);
+          grew |= mn > m[n][i];
+          m[n][i] = mn;
+        }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            l[n][i] *= shrink[n][i];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              o[mt][n][i] *= shrink[n][i];
+              o[mt][n][2 + i] *= shrink[n][i];
+            }
+          }
+      }
+      uint32_t pb[2][NT][2];  // weights as the column operand of the two 16-key steps
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float x = exp2f(s[mt][n][2 * h] - safe[n][0]), y = exp2f(s[mt][n][2 * h + 1] - safe[n][1]);
+            l[n][0] += x;
+            l[n][1] += y;
+            pb[mt][n][h] = transpose8x8(pack_bf16x2(x, y));
+          }
+      {
+        const int mi = lane >> 3, r = lane & 7, key = (mi >> 1) * 8 + r;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            uint32_t va[4];
+            const int ch = 2 * mt + (mi & 1);
+            ldsm_x4_t(va, vs_addr + (ch >> 3) * (BT * 128) + (kt * 16 + key) * 128 + (((ch & 7) ^ r) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_bf16(o[mt][n], va, pb[kt][n][0], pb[kt][n][1]);
+          }
+      }
+      st = next_stage(st, 1);
+    }
+    // given up: the copies in flight must land before the shared memory changes hands
+    for (; used != begun; ++used) mbar_wait(smem_u32(&full_s[warp][used % C::STAGES]), (used / C::STAGES) & 1, nullptr, err, 2 * kWaitLimitNs);
+    __syncthreads();  // the rings are free: the warps' sums take their place
+    float* so = reinterpret_cast<float*>(smem);
+    float* sm = so + 4 * 8 * NT * C::OP;
+    float* sl = sm + 4 * 8 * NT;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int rl = warp * 8 * NT + 8 * n + 2 * t + i;
+        const float lt = sum_over_keys(l[n][i]);
+        if (g == 0) {
+          sm[rl] = m[n][i];
+          sl[rl] = lt;
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          so[rl * C::OP + 16 * mt + g] = o[mt][n][i];
+          so[rl * C::OP + 16 * mt + 8 + g] = o[mt][n][2 + i];
+        }
+      }
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(8 * NT, rows) * (HDP / 4); i += kAttnThreads) {
+      const int rl = i / (HDP / 4), c = (i % (HDP / 4)) * 4;
+      if (c >= d.head_dim) continue;
+      float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w * 8 * NT + rl]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = exp2f(sm[w * 8 * NT + rl] - base);
+        const float4 x = *reinterpret_cast<const float4*>(so + (w * 8 * NT + rl) * C::OP + c);
+        sum = fmaf(f, sl[w * 8 * NT + rl], sum);
+        acc.x = fmaf(f, x.x, acc.x); acc.y = fmaf(f, x.y, acc.y); acc.z = fmaf(f, x.z, acc.z); acc.w = fmaf(f, x.w, acc.w);
+      }
+      if (whole) {
+        const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
+        const int tok = rq.q0 + rl / a.group, head = e * a.group + rl % a.group;
+        uint2 v;
+        v.x = pack_bf16x2(acc.x * inv, acc.y * inv);
+        v.y = pack_bf16x2(acc.z * inv, acc.w * inv);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (long long)tok * d.out_stride + (long long)head * d.head_dim + c) = v;
+        if (a.lse && c == 0) a.lse[(long long)tok * d.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
+      } else {
+        const long long at = slot * C::ROWS + rl;
+        *reinterpret_cast<float4*>(a.part_o + at * HDP + c) = acc;
+        if (c == 0) {
+          a.part_m[at] = top;
+          a.part_l[at] = sum;
+        }
+      }
+    }
+    fence_proxy_async_smem();  // the next piece's copies overwrite what was read and written here
+    __syncthreads();
+  };
+  split_walk<BT>(a, piece, [&](int b, const Request& rq, int e, int c0, int c1) { join_pieces<__nv_bfloat16, HDP, C::ROWS>(a, b, e, rq, c0, c1); });
 }
 
 // a block per row tile (x), key head (y) and share of its keys (z)
@@ -485,78 +846,6 @@ __global__ void __launch_bounds__(kJoinThreads) attn_chunk_join_kernel(const Att
   }
 }
 
-// Adds the partial sums of every tile that several blocks share, in block order. A block per
-// (key head, request); a row is given to one or several warps, which take its pieces in turn.
-template <typename T, int HDP, int WM>
-__global__ void __launch_bounds__(kJoinThreads) attn_join_kernel(const AttnArgs a, int split_blocks) {
-  pdl_wait();
-  pdl_trigger();
-  constexpr int ROWS = 16 * WM, NW = kJoinThreads / 32, V = HDP / 32;
-  __shared__ float part[NW][HDP + 2];
-  const mdlc_attn_desc& d = a.d;
-  const int e = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long units = a.first_unit[d.batch], u0 = a.first_unit[b];
-  const long long n = (a.first_unit[b + 1] - u0) / d.kv_heads;
-  if (n == 0) return;
-  const int blocks = (int)min((long long)split_blocks, units);
-  const int c0 = block_of(u0 + e * n, units, blocks), c1 = block_of(u0 + (e + 1) * n - 1, units, blocks);
-  if (c0 == c1) return;
-  const Request rq = request_of(a, b);
-  const int rows = rq.q_len * a.group;
-  int wpr = 1;  // warps of a row
-  while (wpr * 2 * rows <= NW) wpr *= 2;
-  const int rpb = NW / wpr;
-  for (int rb = 0; rb < rows; rb += rpb) {
-    const int r = rb + warp / wpr, w = warp % wpr;
-    float top = -INFINITY, sum = 0.0f, acc[V] = {};
-    if (r < rows) {
-#pragma unroll 4
-      for (int c = c0 + w; c <= c1; c += wpr) {
-        const long long at = ((long long)b * d.kv_heads + e + c) * ROWS + r;
-        const float pm = a.part_m[at], pl = a.part_l[at];
-        float x[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] = a.part_o[at * HDP + i * 32 + lane];
-        const float mn = fmaxf(top, pm), safe = mn == -INFINITY ? 0.0f : mn;
-        const float f0 = exp2f(top - safe), f1 = exp2f(pm - safe);
-        top = mn;
-        sum = sum * f0 + pl * f1;
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = acc[i] * f0 + x[i] * f1;
-      }
-    }
-    if (wpr > 1) {
-      __syncthreads();
-      if (lane == 0) {
-        part[warp][HDP] = top;
-        part[warp][HDP + 1] = sum;
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) part[warp][i * 32 + lane] = acc[i];
-      __syncthreads();
-      if (w == 0) {
-        for (int k = 1; k < wpr; ++k) {
-          const float pm = part[warp + k][HDP], mn = fmaxf(top, pm), safe = mn == -INFINITY ? 0.0f : mn;
-          const float f0 = exp2f(top - safe), f1 = exp2f(pm - safe);
-          top = mn;
-          sum = sum * f0 + part[warp + k][HDP + 1] * f1;
-#pragma unroll
-          for (int i = 0; i < V; ++i) acc[i] = acc[i] * f0 + part[warp + k][i * 32 + lane] * f1;
-        }
-      }
-    }
-    if (w == 0 && r < rows) {
-      const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
-      const int tok = rq.q0 + r / a.group, head = e * a.group + r % a.group;
-      T* po = static_cast<T*>(a.out) + (long long)tok * d.out_stride + (long long)head * d.head_dim;
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i * 32 + lane < d.head_dim) store_out<T>(po + i * 32 + lane, acc[i] * inv);
-      if (a.lse && lane == 0) a.lse[(long long)tok * d.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
-    }
-  }
-}
-
 // ------------------------------------------------------------ host
 int padded_dim(int head_dim) { return head_dim <= 64 ? 64 : 128; }
 
@@ -592,7 +881,7 @@ Chunk chunk_of(const mdlc_attn_desc& d) {
 }
 
 struct Layout {
-  size_t part_o, part_m, part_l, first_unit, total;
+  size_t part_o, part_m, part_l, total;
 };
 Layout layout_of(const mdlc_attn_desc& d) {
   const size_t slots = (size_t)d.batch * d.kv_heads + kMaxBlocks;
@@ -604,8 +893,7 @@ Layout layout_of(const mdlc_attn_desc& d) {
   l.part_o = 0;
   l.part_m = align256(rows * padded_dim(d.head_dim) * 4);
   l.part_l = l.part_m + align256(rows * 4);
-  l.first_unit = l.part_l + align256(rows * 4);
-  l.total = l.first_unit + align256(((size_t)d.batch + 1) * 8);
+  l.total = l.part_l + align256(rows * 4);
   return l;
 }
 
@@ -628,24 +916,48 @@ template <typename T, int HDP, int WM>
 cudaError_t run_split(mdlc_ctx* ctx, const AttnArgs& a) {
   const int smem = Cfg<T, HDP, WM>::SMEM;
   auto* kern = attn_split_kernel<T, HDP, WM>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static SmemLimit seen;
+  const cudaError_t e = allow_smem(seen, ctx->device, kern, smem);
   if (e != cudaSuccess) return e;
   // one or two blocks per SM, as shared memory allows
   const int blocks = min(kMaxBlocks, ctx->num_sms * (smem <= 100 * 1024 ? 2 : 1));
   mdlc_note_launch(ctx);
-  e = launch_pdl(kern, dim3(blocks), dim3(kAttnThreads), smem, ctx->stream, a, ctx->d_err);
-  if (e != cudaSuccess) return e;
-  mdlc_note_launch(ctx);
-  return launch_pdl(attn_join_kernel<T, HDP, WM>, dim3(a.d.kv_heads, a.d.batch), dim3(kJoinThreads), 0, ctx->stream, a, blocks);
+  return launch_pdl(kern, dim3(blocks), dim3(kAttnThreads), smem, ctx->stream, a, ctx->d_err);
 }
+
+template <int HDP, int NT>
+cudaError_t run_narrow(mdlc_ctx* ctx, const AttnArgs& a) {
+  using C = NarrowCfg<HDP, NT>;
+  CUtensorMap maps[2];
+  cudaError_t e = attn_tensor_maps(a, min(a.d.page, C::BT), &maps[0], &maps[1]);
+  if (e != cudaSuccess) return e;
+  static SmemLimit seen;
+  e = allow_smem(seen, ctx->device, attn_narrow_kernel<HDP, NT>, C::SMEM);
+  if (e != cudaSuccess) return e;
+  const int blocks = min(kMaxBlocks, ctx->num_sms * (C::SMEM <= 100 * 1024 ? 2 : 1));
+  mdlc_note_launch(ctx);
+  return launch_pdl(attn_narrow_kernel<HDP, NT>, dim3(blocks), dim3(kAttnThreads), C::SMEM, ctx->stream, a, maps[0], maps[1], ctx->d_err);
+}
+
+// pages of 8, 16, 32, ... keys
+bool narrow_fits(const mdlc_attn_desc& d) { return d.dtype == MDLC_BF16 && d.page >= 8 && (d.page & (d.page - 1)) == 0; }
 
 template <typename T, int HDP>
 cudaError_t run_attn(mdlc_ctx* ctx, AttnArgs& a) {
   const int wm = split_groups(a.d);
   cudaError_t e = cudaSuccess;
-  if (wm == 1) e = run_split<T, HDP, 1>(ctx, a);
-  else if (wm == 2) e = run_split<T, HDP, 2>(ctx, a);
-  else if (wm == 4) e = run_split<T, HDP, 4>(ctx, a);
+  if (wm == 1 && narrow_fits(a.d)) {
+    // requests of up to 8 rows in one column tile; with more than 8 heads per key head, or several tokens, two
+    const bool one = a.group <= 8 && ((long long)a.d.max_q * a.group <= 8 || (long long)a.d.max_q * a.group > 16);
+    if (one) a.split_rows = 8;
+    e = one ? run_narrow<HDP, 1>(ctx, a) : run_narrow<HDP, 2>(ctx, a);
+  } else if (wm == 1) {
+    e = run_split<T, HDP, 1>(ctx, a);
+  } else if (wm == 2) {
+    e = run_split<T, HDP, 2>(ctx, a);
+  } else if (wm == 4) {
+    e = run_split<T, HDP, 4>(ctx, a);
+  }
   const Chunk c = chunk_of(a.d);
   if (e != cudaSuccess || !c.used) return e;
   a.splits = c.splits;
@@ -655,7 +967,8 @@ cudaError_t run_attn(mdlc_ctx* ctx, AttnArgs& a) {
     e = attn_tc_launch(ctx, a, grid);
   } else {
     const int smem = Cfg<T, HDP, 4>::SMEM;
-    e = cudaFuncSetAttribute(attn_chunk_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static SmemLimit seen;
+    e = allow_smem(seen, ctx->device, attn_chunk_kernel<T, HDP>, smem);
     if (e == cudaSuccess) e = launch_pdl(attn_chunk_kernel<T, HDP>, grid, dim3(kAttnThreads), smem, ctx->stream, a, ctx->d_err);
   }
   if (e != cudaSuccess || c.splits == 1) return e;
@@ -704,7 +1017,7 @@ extern "C" int mdlc_paged_attn(mdlc_ctx* ctx, const mdlc_attn_desc* desc, const 
   a.part_o = reinterpret_cast<float*>(ws + l.part_o);
   a.part_m = reinterpret_cast<float*>(ws + l.part_m);
   a.part_l = reinterpret_cast<float*>(ws + l.part_l);
-  a.first_unit = reinterpret_cast<long long*>(ws + l.first_unit);
+  a.arrived = ctx->d_attn_cnt;
   const bool bf16 = desc->dtype == MDLC_BF16;
   cudaError_t e;
   if (padded_dim(desc->head_dim) == 64) e = bf16 ? run_attn<__nv_bfloat16, 64>(ctx, a) : run_attn<float, 64>(ctx, a);

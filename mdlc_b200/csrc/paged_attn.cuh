@@ -17,15 +17,17 @@ struct AttnArgs {
   int split_rows;     // requests with at most this many rows go to split mode
   int splits;         // chunk mode: blocks that may share a row tile's keys
   float scale_log2;   // scale * log2(e)
-  // workspace: partial sums [slot][rows][hdp], their maxima (base-2 exponent) and sums [slot][rows], first unit of each request
+  // workspace: partial sums [slot][rows][hdp], their maxima (base-2 exponent) and sums [slot][rows]
   float *part_o, *part_m, *part_l;
-  long long* first_unit;  // [batch + 1]
+  int* arrived;           // split mode: arrivals at the tile that starts in block c and others share
 };
 
 // chunk mode on the tensor cores' tcgen05 form (bf16): rows of a tile, keys of a block
 constexpr int kTcRows = 256, kTcKeys = 128;
 bool attn_tc_fits(const mdlc_attn_desc& d);
 cudaError_t attn_tc_launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid);
+// tensor maps of the two caches (rows of head_dim elements) with boxes of `box` rows x 64 columns, 128-byte swizzle
+cudaError_t attn_tensor_maps(const AttnArgs& a, int box, CUtensorMap* k, CUtensorMap* v);
 
 // ------------------------------------------------------------ one request's geometry
 struct Request {

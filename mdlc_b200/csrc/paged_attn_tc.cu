@@ -20,6 +20,7 @@
 // last page's tail of the values is cleared in shared memory (its cache slots may hold NaN, and 0 x NaN
 // would reach every row).
 #include "conv.h"
+#include "func_attr.h"
 #include "paged_attn.cuh"
 
 namespace mdlc {
@@ -439,25 +440,30 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
 
 template <int HDP>
 cudaError_t launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid) {
-  const auto encode = tensor_map_encoder();
-  if (!encode) return cudaErrorNotSupported;
-  const mdlc_attn_desc& d = a.d;
-  // a cache as rows of head_dim elements, one per (page, key head, token)
-  const cuuint64_t dims[2] = {(cuuint64_t)d.head_dim, (cuuint64_t)d.pages * d.kv_heads * d.page};
-  const cuuint64_t strides[1] = {(cuuint64_t)d.head_dim * 2};
-  const cuuint32_t box[2] = {64, (cuuint32_t)min(d.page, kKeys)}, steps[2] = {1, 1};
   CUtensorMap maps[2];
-  for (int i = 0; i < 2; ++i)
-    if (encode(&maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(i ? a.v : a.k), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return cudaErrorInvalidValue;
-  const cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel<HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, TcCfg<HDP>::SMEM);
+  cudaError_t e = attn_tensor_maps(a, min(a.d.page, kKeys), &maps[0], &maps[1]);
+  if (e != cudaSuccess) return e;
+  static SmemLimit seen;
+  e = allow_smem(seen, ctx->device, attn_tc_kernel<HDP>, TcCfg<HDP>::SMEM);
   if (e != cudaSuccess) return e;
   // key heads fastest: the tiles that see the most keys start first in all of them
   return launch_pdl(attn_tc_kernel<HDP>, dim3(grid.y, grid.x, grid.z), dim3(kThreads), TcCfg<HDP>::SMEM, ctx->stream, a, maps[0], maps[1], ctx->d_err);
 }
 
 }  // namespace
+
+cudaError_t attn_tensor_maps(const AttnArgs& a, int box, CUtensorMap* k, CUtensorMap* v) {
+  const auto encode = tensor_map_encoder();
+  if (!encode) return cudaErrorNotSupported;
+  const mdlc_attn_desc& d = a.d;
+  const cuuint64_t dims[2] = {(cuuint64_t)d.head_dim, (cuuint64_t)d.pages * d.kv_heads * d.page}, strides[1] = {(cuuint64_t)d.head_dim * 2};
+  const cuuint32_t size[2] = {64, (cuuint32_t)box}, steps[2] = {1, 1};
+  for (int i = 0; i < 2; ++i)
+    if (encode(i ? v : k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(i ? a.v : a.k), dims, strides, size, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+      return cudaErrorInvalidValue;
+  return cudaSuccess;
+}
 
 // bf16, pages that tile a 128-key block, a positive scale (the running maximum is that of the raw scores)
 bool attn_tc_fits(const mdlc_attn_desc& d) {

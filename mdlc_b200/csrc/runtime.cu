@@ -60,7 +60,9 @@ int mdlc_ctx_create(int device, mdlc_ctx** out) {
       cudaMemset(ctx->d_err, 0, 256) != cudaSuccess || cudaMalloc(&ctx->d_pad, 4096) != cudaSuccess ||
       cudaMalloc(&ctx->d_split_ws, kSplitWsBytes) != cudaSuccess ||
       cudaMalloc(&ctx->d_split_cnt, kSplitCounters * sizeof(int)) != cudaSuccess ||
-      cudaMemset(ctx->d_split_cnt, 0, kSplitCounters * sizeof(int)) != cudaSuccess) {
+      cudaMemset(ctx->d_split_cnt, 0, kSplitCounters * sizeof(int)) != cudaSuccess ||
+      cudaMalloc(&ctx->d_attn_cnt, kAttnCounters * sizeof(int)) != cudaSuccess ||
+      cudaMemset(ctx->d_attn_cnt, 0, kAttnCounters * sizeof(int)) != cudaSuccess) {
     delete ctx;
     return MDLC_ERR_CUDA;
   }
@@ -95,6 +97,7 @@ int mdlc_ctx_destroy(mdlc_ctx* ctx) {
   cudaFree(ctx->d_pad);
   cudaFree(ctx->d_split_ws);
   cudaFree(ctx->d_split_cnt);
+  cudaFree(ctx->d_attn_cnt);
   cudaEventDestroy(ctx->order);
   cudaStreamDestroy(ctx->own_stream);
   if (ctx->copy_stream) cudaStreamDestroy(ctx->copy_stream);

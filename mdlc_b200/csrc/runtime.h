@@ -28,6 +28,8 @@ struct mdlc_ctx {
   // conv call allocates (calls may be captured in a CUDA graph)
   uint32_t* d_split_ws = nullptr;
   int* d_split_cnt = nullptr;
+  // paged attention: arrivals at the tiles that several blocks share (kept at zero between calls: the last one resets)
+  int* d_attn_cnt = nullptr;
   cudaGraph_t graph = nullptr;
   cudaGraphExec_t graph_exec = nullptr;
   bool capturing = false;
@@ -43,6 +45,7 @@ int mdlc_cuda_status(mdlc_ctx* ctx, cudaError_t e, const char* what);
 
 constexpr size_t kSplitWsBytes = 8u << 20;  // split-K partials: 64 units of 128 x 256 fp32
 constexpr int kSplitCounters = 1024;
+constexpr int kAttnCounters = 512;
 
 inline void mdlc_note_launch(mdlc_ctx* ctx) {
   if (ctx->capturing)
