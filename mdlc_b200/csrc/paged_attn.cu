@@ -25,6 +25,9 @@ namespace {
 constexpr int kAttnThreads = 128;
 constexpr int kStages = 3;
 constexpr int kUnit = 128;      // keys of one unit of split work
+// What beginning and ending a tile costs, in units: without it a block whose share is many short requests ends long after
+// the others (64 requests of 64 to 8192 keys: the last SM 271k cycles, the mean 189k)
+constexpr int kTileCost = 2;
 constexpr int kMaxBlocks = 512; // split-mode blocks at most (bounds the workspace)
 constexpr int kJoinThreads = 256;
 constexpr int kLeastKeys = 256; // keys of a share of a chunk tile at least
@@ -448,7 +451,7 @@ MDLC_DEV void split_walk(const AttnArgs& a, Piece piece, Join join) {
     const Request r = request_of(a, b);
     const long long rows = (long long)r.q_len * a.group;
     if (rows == 0 || rows > a.split_rows) return 0;
-    return max(1, (span_of(a, r, 0, r.q_len - 1, BT).n + UB - 1) / UB);
+    return kTileCost + max(1, (span_of(a, r, 0, r.q_len - 1, BT).n + UB - 1) / UB);
   };
   const int per = (d.batch + kAttnThreads - 1) / kAttnThreads;
   const int b0 = min((int)threadIdx.x * per, d.batch), b1 = min(b0 + per, d.batch);
@@ -475,18 +478,21 @@ MDLC_DEV void split_walk(const AttnArgs& a, Piece piece, Join join) {
   while (u0 < u1) {
     const Request rq = request_of(a, pl.b);
     const long long n = units_of(pl.b);
-    if (u0 >= pl.first + n * d.kv_heads) {
+    if (u0 >= pl.first + n * d.kv_heads) {  // (n is 0 for a request that is not split mode's)
       pl.first += n * d.kv_heads;
       ++pl.b;
       continue;
     }
     const int e = (int)((u0 - pl.first) / n);
-    const long long tile0 = pl.first + e * n, end = min(u1, tile0 + n);
-    const Span sp = span_of(a, rq, 0, rq.q_len - 1, BT);
-    const int blk0 = (int)(u0 - tile0) * UB, blk1 = min((int)(end - tile0) * UB, sp.n);
-    const bool whole = u0 == tile0 && end == tile0 + n;
-    piece(pl.b, rq, e, sp, blk0, blk1, whole, (long long)pl.b * d.kv_heads + e + blockIdx.x);
-    if (!whole) join(pl.b, rq, e, block_of(tile0, total, blocks), block_of(tile0 + n - 1, total, blocks));
+    // the tile's keys begin kTileCost units after its place on the line; a share that ends before them has none of them
+    const long long tile0 = pl.first + e * n + kTileCost, end = min(u1, tile0 + n - kTileCost), from = max(u0, tile0);
+    if (from < end) {
+      const Span sp = span_of(a, rq, 0, rq.q_len - 1, BT);
+      const int blk0 = (int)(from - tile0) * UB, blk1 = min((int)(end - tile0) * UB, sp.n);
+      const bool whole = from == tile0 && end == tile0 + n - kTileCost;
+      piece(pl.b, rq, e, sp, blk0, blk1, whole, (long long)pl.b * d.kv_heads + e + blockIdx.x);
+      if (!whole) join(pl.b, rq, e, block_of(tile0, total, blocks), block_of(tile0 + n - kTileCost - 1, total, blocks));
+    }
     u0 = end;
   }
 }
@@ -511,11 +517,12 @@ __global__ void __launch_bounds__(kAttnThreads) attn_split_kernel(const AttnArgs
 // operands turned. The 16 rows of a product are keys (S^T = K Q^T) or output columns (O^T = V^T P^T) and the 8 columns are
 // the tile's rows, so that 8 rows cost half the products, registers and exponentials that 16 would; the weights go
 // from the first product's result to the second one's operand through movmatrix, the 8 x 8 transpose.
-// Every warp has its own ring of 32-key blocks, filled by TMA (a box per page and 64 columns, issued
+// Every warp has its own ring of 16- or 32-key blocks, filled by TMA (a box per page and 64 columns, issued
 // by as many lanes). Bounded by the cache's bytes: NARROW_FIGURES.
 template <int HDP, int NT>
 struct NarrowCfg {
-  static constexpr int BT = 32, ROWS = 16;                 // workspace slots hold 16 rows
+  static constexpr int BT = HDP == 128 ? 16 : 32;          // two blocks per SM: one streams while the other begins or ends a tile
+  static constexpr int ROWS = 16;                          // workspace slots hold 16 rows
   static constexpr int TILE = BT * HDP * 2;                // keys or values of a block
   static constexpr int STAGES = 3;
   static constexpr int RING = 4 * STAGES * 2 * TILE;
@@ -542,7 +549,7 @@ template <int HDP, int NT>
 __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                                                                       const __grid_constant__ CUtensorMap vmap, int* err) {
   using C = NarrowCfg<HDP, NT>;
-  constexpr int BT = C::BT, HALVES = HDP / 64, MT = HDP / 16;
+  constexpr int BT = C::BT, HALVES = HDP / 64, MT = HDP / 16, KT = BT / 16;
   extern __shared__ unsigned char narrow_raw[];
   __shared__ __align__(8) uint64_t full_s[4][C::STAGES];
   unsigned char* smem = narrow_raw + ((1024 - (smem_u32(narrow_raw) & 1023)) & 1023);
@@ -643,13 +650,13 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
         __syncwarp();
       }
       // scores: 16-key tile mt, rows 8 n + 2 t
-      float s[2][NT][4] = {};
+      float s[KT][NT][4] = {};
       {
         const int mi = lane >> 3, r = lane & 7, key = (mi & 1) * 8 + r;
 #pragma unroll
         for (int ks = 0; ks < MT; ++ks)
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
+          for (int mt = 0; mt < KT; ++mt) {
             uint32_t ka[4];
             const int ch = 2 * ks + (mi >> 1);
             ldsm_x4(ka, ks_addr + (ch >> 3) * (BT * 128) + (mt * 16 + key) * 128 + (((ch & 7) ^ r) << 4));
@@ -667,7 +674,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
         for (int i = 0; i < 2; ++i) {
           float top = -INFINITY;
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
+          for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float x = s[mt][n][2 * h + i] * a.scale_log2;
@@ -698,9 +705,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
             }
           }
       }
-      uint32_t pb[2][NT][2];  // weights as the column operand of the two 16-key steps
+      uint32_t pb[KT][NT][2];  // weights as the column operand of the 16-key steps
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < KT; ++mt)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -713,7 +720,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
       {
         const int mi = lane >> 3, r = lane & 7, key = (mi >> 1) * 8 + r;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
             uint32_t va[4];
