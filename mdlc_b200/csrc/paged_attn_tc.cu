@@ -9,10 +9,10 @@
 //   warp 8          issues every MMA (one thread) and owns the tensor memory
 //   warp 9          loads keys and values by TMA, a box per page, 32 lanes at once
 //   (warps 8-11 give registers to the softmax warpgroups; 10 and 11 do nothing else)
-// Tensor memory (512 columns): scores of the two tiles [0, 256), the weights over the first half of
-// their own tile's scores; outputs [256, 256 + 2 HDP). The MMA order per key block j is
-// O0 += P0(j) V(j), S0 = Q0 K(j+1), O1 += P1(j) V(j), S1 = Q1 K(j+1): while one tile's products run,
-// the other tile's weights are computed. Issue order makes S0(j+1) overwrite P0(j) only after it was read.
+// Tensor memory (512 columns): scores of the two tiles [0, 256), 64 columns per half of a key block, the weights over the
+// first 32 of their own half's; outputs [256, 256 + 2 HDP). Per half n of a key block the MMAs are O += P(n) V(n), then the scores of
+// half n + 2 into the place that P(n) leaves (issue order makes them overwrite it only after it was read): a tile always has the next half's
+// scores waiting, so its softmax does not wait for its own products.
 // Outputs stay in tensor memory; they are rescaled only when a row's maximum grows by more than 2^8
 // over the one in use (weights are then at most 2^8; bf16 rounding is relative, so nothing is lost),
 // which after the first blocks hardly happens.
@@ -44,8 +44,8 @@ struct TcCfg {
   static constexpr int SMEM = BARS + 256 + 1024;        // 1024: alignment of the base
   static constexpr int O_COL = 256;
 };
-// barriers
-enum { kFull = 0, kEmpty = kRing, kRaw = 2 * kRing, kQ, kS0, kS1, kP0, kP1, kO0, kO1, kDrain, kBars };
+// barriers; scores, weights and outputs have one per row tile and half of the key block (kS + 2 tile + half, ...)
+enum { kFull = 0, kEmpty = kRing, kRaw = 2 * kRing, kQ, kS, kP = kS + 4, kO = kP + 4, kDrain = kO + 4, kBars };
 
 // instruction descriptor: bf16 x bf16 -> fp32; B stored along its N axis (values)
 constexpr uint32_t idesc_bf16_nmajor(int M, int N) { return idesc_bf16(M, N) | (1u << 16); }
@@ -56,12 +56,36 @@ MDLC_DEV uint64_t umma_desc_sw128_n(uint32_t saddr, uint32_t lbo_bytes) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo_bytes >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-// A operand in tensor memory
-MDLC_DEV void umma_bf16_ta(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// MMAs and commits issued by the lane that `leader` marks while the whole warp walks the loop: with operands that are
+// uniform over the warp the descriptors stay in uniform registers (issued from a branch of one lane, an MMA took
+// 112 cycles whatever its size, and the tensor pipe idled half of the time)
+MDLC_DEV uint32_t elect_leader() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is;
+}
+MDLC_DEV void umma_lead(uint32_t leader, uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+// A operand in tensor memory
+MDLC_DEV void umma_lead_ta(uint32_t leader, uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+      : "memory");
+}
+MDLC_DEV void commit_lead(uint32_t leader, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader)
       : "memory");
 }
 #define MDLC_R8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
@@ -109,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
   __shared__ long long warp_sums[kThreads / 32];
   __shared__ Place place_s;
   __shared__ uint32_t tmem_s;
-  __shared__ int abort_s;
+  __shared__ int abort_s, missing_s;
   unsigned char* smem = tc_smem_raw + ((1024 - (smem_u32(tc_smem_raw) & 1023)) & 1023);
   const uint32_t sbase = smem_u32(smem);
   auto bar = [&](int i) { return sbase + C::BARS + 8 * i; };
@@ -140,13 +164,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
     }
     mbar_init(bar(kRaw), 1);
     mbar_init(bar(kQ), 256);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(kS0 + i), 1);
-      mbar_init(bar(kP0 + i), 128);
-      mbar_init(bar(kO0 + i), 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(bar(kS + i), 1);
+      mbar_init(bar(kP + i), 128);
+      mbar_init(bar(kO + i), 1);
     }
     mbar_init(bar(kDrain), 1);
-    abort_s = 0;
+    abort_s = missing_s = 0;
     fence_mbar_init();
   }
   if (warp == 8) {
@@ -156,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_s;
+  const uint32_t tmem = tmem_s;  // all 512 columns: 0, which the MMA warp takes for granted
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax
@@ -165,17 +189,39 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
     {
       const int chunks = d.head_dim / 8;
       constexpr int CH = HDP / 8;
-      for (int i = threadIdx.x; i < kRows * CH; i += 256) {
-        const int rl = i / CH, c = i % CH, r = t.r0 + rl;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < t.rows && c < chunks)
-          v = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + (long long)(t.rq.q0 + r / a.group) * d.q_stride +
-                                                   (long long)(e * a.group + r % a.group) * d.head_dim) + c);
-        *reinterpret_cast<uint4*>(smem + C::Q + (rl >> 7) * C::TILE + (c >> 3) * 16384 + (rl & 127) * 128 + (((c & 7) ^ (rl & 7)) << 4)) = v;
+      for (int i0 = threadIdx.x; i0 < kRows * CH; i0 += 8 * 256) {  // eight loads at a time
+        uint4 v[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const int i = i0 + n * 256, rl = i / CH, c = i % CH, r = t.r0 + rl;
+          v[n] = make_uint4(0, 0, 0, 0);
+          if (r < t.rows && c < chunks)
+            v[n] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + (long long)(t.rq.q0 + r / a.group) * d.q_stride +
+                                                        (long long)(e * a.group + r % a.group) * d.head_dim) + c);
+        }
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+          const int i = i0 + n * 256, rl = i / CH, c = i % CH;
+          *reinterpret_cast<uint4*>(smem + C::Q + (rl >> 7) * C::TILE + (c >> 3) * 16384 + (rl & 127) * 128 + (((c & 7) ^ (rl & 7)) << 4)) = v[n];
+        }
       }
       fence_proxy_async_smem();
       mbar_arrive(bar(kQ));
     }
+    // Ids that do not exist hide their keys: looked for once, so that the blocks need not look (a load from the table
+    // in front of every block cost 570 cycles of 4200)
+    auto missing = [&](int j) {
+      return j < sp.hi && (j + min(d.page, kKeys) > sp.lo || j < d.sinks) &&
+             (unsigned)__ldg(a.table + (long long)t.b * d.table_stride + j / d.page) >= (unsigned)d.pages;
+    };
+    {
+      const int per = kKeys / min(d.page, kKeys);
+      bool none = false;
+      for (int i = threadIdx.x; i < nb * per; i += 256) none |= missing(key_of_block(sp, blk0 + i / per, kKeys) + i % per * min(d.page, kKeys));
+      if (none) missing_s = 1;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+    }
+    const bool any_missing = *(volatile int*)&missing_s;
     const int tile = warp >> 2, rl = threadIdx.x, r = t.r0 + rl;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + tile * 128, o_addr = tmem + lanes + C::O_COL + tile * HDP;
@@ -187,65 +233,63 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     if (tile < n_tiles) {
-      // page ids of a block, a lane each, to notice ids that do not exist (their keys are hidden)
-      const int box = min(d.page, kKeys), boxes = kKeys / box, box_log2 = 31 - __clz(box);  // a power of two
-      auto id_of = [&](int blk) {
-        int bad = 0;
-        if (lane < boxes && blk < blk1) {
-          const int j = key_of_block(sp, blk, kKeys) + lane * box;
-          if (j < sp.hi && (j + box > sp.lo || j < d.sinks))
-            bad = (unsigned)__ldg(a.table + (long long)t.b * d.table_stride + j / d.page) >= (unsigned)d.pages;
-        }
-        return bad;
-      };
-      int bad_next = id_of(blk0);
-      for (int j = 0; j < nb; ++j) {
-        const int base = key_of_block(sp, blk0 + j, kKeys);
-        const uint32_t bad = __ballot_sync(0xffffffffu, bad_next);
-        bad_next = id_of(blk0 + j + 1);
-        ok = mbar_wait(bar(kS0 + tile), j & 1, abort_flag, err, kWaitCycles);
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
-        }
+      const int box = min(d.page, kKeys), box_log2 = 31 - __clz(box);  // keys of a TMA box, a power of two
+      // blocks [open0, open1) of this share are seen whole by every row of the tile: no mask
+      int open0 = 0, open1 = nb;
+      if (any_missing) open1 = 0;
+      while (open1 > 0 && key_of_block(sp, blk0 + open1 - 1, kKeys) + kKeys - 1 > p_min) --open1;
+      if (d.window > 0)
+        while (open0 < open1 && key_of_block(sp, blk0 + open0, kKeys) <= p_max - d.window) ++open0;
+      for (int n = 0; n < 2 * nb; ++n) {
+        const int j = n >> 1, h = n & 1;
+        const uint32_t sh = s_addr + 64 * h;  // this half's scores, and their weights
+        ok = __all_sync(0xffffffffu, mbar_wait(bar(kS + 2 * tile + h), j & 1, abort_flag, err, kWaitCycles));
+        if (!ok) break;
         tc_fence_after();
-        // a block that every row of the tile sees whole needs no mask
-        const bool open = bad == 0 && base + kKeys - 1 <= p_min && (d.window == 0 || base > p_max - d.window || base + kKeys <= d.sinks);
-        const int hi = p - base, lo = d.window > 0 ? hi - d.window : -1, kept = d.window > 0 ? d.sinks - base : 0;
-        if (!open) {
+        if (j < open0 || j >= open1) {
           // hidden keys to -inf, in place (a loop of its own, so that the common path stays small)
+          const int base = key_of_block(sp, blk0 + j, kKeys) + 64 * h;
+          const int hi = p - base, lo = d.window > 0 ? hi - d.window : -1, kept = d.window > 0 ? d.sinks - base : 0;
+          uint32_t bad = 0;  // boxes of this block without a page
+          if (any_missing) bad = __ballot_sync(0xffffffffu, lane < (kKeys >> box_log2) && missing(base - 64 * h + (lane << box_log2)));
+          // bits [0, n) of a word, n of any sign or size
+          auto below = [](int n) { return n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u); };
 #pragma unroll 1
-          for (int k0 = 0; k0 < kKeys; k0 += 32) {
+          for (int k0 = 0; k0 < 64; k0 += 32) {
+            uint32_t see = below(hi + 1 - k0) & (~below(lo + 1 - k0) | below(kept - k0));
+            if (bad) {
+#pragma unroll 1
+              for (int i = 0; i < 32; i += 8)
+                if ((bad >> ((64 * h + k0 + i) >> box_log2)) & 1u) see &= ~(0xffu << i);
+            }
             uint32_t s[32];
-            tmem_ld32(s_addr + k0, s);
+            tmem_ld32(sh + k0, s);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const bool seen = k0 + i <= hi && (k0 + i > lo || k0 + i < kept) && !((bad >> ((k0 + i) >> box_log2)) & 1u);
-              s[i] = seen ? s[i] : 0xff800000u;
-            }
-            tmem_st32(s_addr + k0, s);
+            for (int i = 0; i < 32; ++i) s[i] = (see >> i) & 1u ? s[i] : 0xff800000u;
+            tmem_st32(sh + k0, s);
           }
           tmem_st_wait();
         }
-        // One pass takes the weights against the maximum in use and the block's own maximum; when that has grown
-        // by more than 2^8 for some row of the warp (or a row sees its first keys) the pass is
-        // repeated with the new one. The weights wait in registers: their place is the scores' own.
-        uint32_t w[64];
+        // One pass takes the weights against the maximum in use and the half's own maximum; when that has grown by more
+        // than 2^8 for some row of the warp (or a row sees its first keys) the pass is repeated with the new one. The
+        // weights wait in registers: their place is the scores' own.
+        uint32_t w[32];
         for (;;) {
           const float mc = m == -INFINITY ? 0.0f : m * c;
           const float2 c2 = splat2(c), mc2 = splat2(-mc);
           float top[2] = {-INFINITY, -INFINITY};
           float2 sum[2] = {splat2(0.0f), splat2(0.0f)};
           uint32_t s[2][32];
-          tmem_ld32(s_addr, s[0]);
+          tmem_ld32(sh, s[0]);
+          tmem_ld_wait();
+          tmem_ld32(sh + 32, s[1]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            tmem_ld_wait();
-            if (k < 3) tmem_ld32(s_addr + 32 * (k + 1), s[(k + 1) & 1]);
+          for (int k = 0; k < 2; ++k) {
+            if (k) tmem_ld_wait();
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              const float2 x = make_float2(__uint_as_float(s[k & 1][i]), __uint_as_float(s[k & 1][i + 1]));
+              const float2 x = make_float2(__uint_as_float(s[k][i]), __uint_as_float(s[k][i + 1]));
               top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], x.x, x.y);
               float2 y = fma2(x, c2, mc2);
               y = make_float2(ex2(y.x), ex2(y.y));
@@ -259,12 +303,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
             l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             break;
           }
-          // a row that has summed nothing yet (sum and output are zero) takes the maximum as it is
-          const float f = grow ? ex2((m - mn) * c) : 1.0f;
+          // a row that has summed nothing yet takes the maximum as it is
+          const float f = fresh ? 0.0f : (grow ? ex2((m - mn) * c) : 1.0f);
           if (fresh || grow) m = mn;
+          l *= f;
           if (__any_sync(0xffffffffu, grow)) {
-            l *= f;
-            ok = mbar_wait(bar(kO0 + tile), (j - 1) & 1, abort_flag, err, kWaitCycles);
+            ok = mbar_wait(bar(kO + 2 * tile + (h ^ 1)), ((n - 1) >> 1) & 1, abort_flag, err, kWaitCycles);  // the half before this one
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
@@ -280,13 +324,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
           }
         }
         if (!ok) break;
-        tmem_st32(s_addr, w);
-        tmem_st32(s_addr + 32, w + 32);
+        tmem_st32(sh, w);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(bar(kP0 + tile));
+        mbar_arrive(bar(kP + 2 * tile + h));
       }
-      if (ok && nb > 0) ok = mbar_wait(bar(kO0 + tile), (nb - 1) & 1, abort_flag, err, kWaitCycles);
+      if (ok && nb > 0) ok = mbar_wait(bar(kO + 2 * tile + 1), (nb - 1) & 1, abort_flag, err, kWaitCycles);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
       if (ok) {
@@ -334,50 +377,56 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
     regs_down<kOtherRegs>();  // warps 8 to 11 alike, before their ways part
     if (warp == 8) {
     // ------------------------------------------------------------ MMA
-    if (lane == 0 && nb > 0) {
-      constexpr uint32_t kIdS = idesc_bf16(128, kKeys), kIdO = idesc_bf16_nmajor(128, HDP);
-      bool ok = mbar_wait(bar(kQ), 0, abort_flag, err, kWaitCycles);
-      auto wait_tile = [&](int u) { return mbar_wait(bar(kFull + u % kRing), (u / kRing) & 1, abort_flag, err, kWaitCycles); };
-      auto scores = [&](int i, int j) {  // S_i = Q_i K(j)^T
-        const uint32_t q = sbase + C::Q + i * C::TILE, k = sbase + C::RING + ((2 * j) % kRing) * C::TILE;
+    const uint32_t leader = elect_leader();
+    const int u_nb = __shfl_sync(0xffffffffu, nb, 0), u_tiles = __shfl_sync(0xffffffffu, n_tiles, 0);
+    if (u_nb > 0) {
+      constexpr uint32_t kIdS = idesc_bf16(128, 64), kIdO = idesc_bf16_nmajor(128, HDP);
+      bool ok = __all_sync(0xffffffffu, mbar_wait(bar(kQ), 0, abort_flag, err, kWaitCycles));
+      auto wait_tile = [&](int u) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar(kFull + u % kRing), (u / kRing) & 1, abort_flag, err, kWaitCycles)); };
+      auto scores = [&](int i, int j, int h) {  // half h of S_i = Q_i K(j)^T
+        const uint32_t q = sbase + C::Q + i * C::TILE, k = sbase + C::RING + ((2 * j) % kRing) * C::TILE + h * 8192;
 #pragma unroll
         for (int ks = 0; ks < HDP / 16; ++ks) {
           const uint32_t off = (ks / 4) * 16384 + (ks % 4) * 32;
-          umma_bf16(tmem + i * 128, umma_desc_sw128(q + off), umma_desc_sw128(k + off), kIdS, ks > 0);
+          umma_lead(leader, i * 128 + h * 64, umma_desc_sw128(q + off), umma_desc_sw128(k + off), kIdS, ks > 0);
         }
-        umma_commit(bar(kS0 + i));
+        commit_lead(leader, bar(kS + 2 * i + h));
       };
       ok = ok && wait_tile(0);
       tc_fence_after();
       if (ok) {
-        for (int i = 0; i < n_tiles; ++i) scores(i, 0);
-        umma_commit(bar(kEmpty + 0));
+        for (int h = 0; h < 2; ++h)
+          for (int i = 0; i < u_tiles; ++i) scores(i, 0, h);
+        commit_lead(leader, bar(kEmpty + 0));
       }
-      for (int j = 0; ok && j < nb; ++j) {
+      for (int j = 0; ok && j < u_nb; ++j) {
         ok = wait_tile(2 * j + 1);
-        for (int i = 0; ok && i < n_tiles; ++i) {
-          ok = mbar_wait(bar(kP0 + i), j & 1, abort_flag, err, kWaitCycles);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t v = sbase + C::RING + ((2 * j + 1) % kRing) * C::TILE;
+        const uint32_t v = sbase + C::RING + ((2 * j + 1) % kRing) * C::TILE;
+        for (int h = 0; ok && h < 2; ++h)
+          for (int i = 0; i < u_tiles; ++i) {
+            ok = __all_sync(0xffffffffu, mbar_wait(bar(kP + 2 * i + h), j & 1, abort_flag, err, kWaitCycles));
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll
-          for (int ks = 0; ks < kKeys / 16; ++ks)
-            umma_bf16_ta(tmem + C::O_COL + i * HDP, tmem + i * 128 + ks * 8, umma_desc_sw128_n(v + ks * 2048, 16384), kIdO, j > 0 || ks > 0);
-          umma_commit(bar(kO0 + i));
-          if (i == n_tiles - 1) umma_commit(bar(kEmpty + (2 * j + 1) % kRing));
-          if (j + 1 < nb) {
-            if (i == 0) {
-              ok = wait_tile(2 * j + 2);
-              if (!ok) break;
-              tc_fence_after();
+            for (int ks = 0; ks < 4; ++ks)
+              umma_lead_ta(leader, C::O_COL + i * HDP, i * 128 + h * 64 + ks * 8, umma_desc_sw128_n(v + (4 * h + ks) * 2048, 16384), kIdO,
+                           j > 0 || h > 0 || ks > 0);
+            commit_lead(leader, bar(kO + 2 * i + h));
+            const bool last = h == 1 && i == u_tiles - 1;
+            if (last) commit_lead(leader, bar(kEmpty + (2 * j + 1) % kRing));
+            if (j + 1 < u_nb) {
+              if (h == 0 && i == 0) {
+                ok = wait_tile(2 * j + 2);
+                if (!ok) break;
+                tc_fence_after();
+              }
+              scores(i, j + 1, h);
+              if (last) commit_lead(leader, bar(kEmpty + (2 * j + 2) % kRing));
             }
-            scores(i, j + 1);
-            if (i == n_tiles - 1) umma_commit(bar(kEmpty + (2 * j + 2) % kRing));
           }
-        }
       }
       // everything issued is done before the tensor memory goes back
-      umma_commit(bar(kDrain));
+      commit_lead(leader, bar(kDrain));
       mbar_wait(bar(kDrain), 0, nullptr, err, kWaitCycles);
     }
     __syncwarp();
