@@ -154,10 +154,17 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page
 // Memory-bound: every element of q, k and v is read and written once. A warp (or
 // a block, when there are few tokens) takes a token; a thread owns one unit of V
 // pairs, reads their cosines and sines once and turns that unit of head after
-// head, kRopeBatch heads' loads in flight at a time. q_out may be q (so loads of a
+// head, kRopeBatch heads' loads in flight at a time, the first ones before the angles are known. q_out may be q (so loads of a
 // batch precede its stores, and no thread reads what another writes).
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
 constexpr int kRopeBatch = 4;
+
+// n / d for 0 <= n < 65536 and 1 <= d <= 65536 as a product: a runtime division costs some 20 instructions
+struct SmallDiv {
+  uint32_t d, m;  // m = floor((2^32 - 1) / d) + 1
+};
+SmallDiv small_div(int d) { return {(uint32_t)d, 0xffffffffu / (uint32_t)d + 1u}; }
+MDLC_DEV int div_small(int n, const SmallDiv& s) { return s.m ? (int)__umulhi((uint32_t)n, s.m) : n; }  // m wraps to 0 for d = 1
 
 struct RopeArgs {
   mdlc_rope_desc d;
@@ -167,6 +174,8 @@ struct RopeArgs {
   const int32_t* slots;
   void *q_out, *k_cache, *v_cache;
   int warps_per_token;
+  SmallDiv units, rest, vals;  // units of a head that turn; vectors of its rest; vectors of a value head
+  int page_shift;              // log2 of the page size, -1: not a power of two
 };
 
 // V elements of T as one load or store of 16, 8 or sizeof(T) bytes
@@ -198,7 +207,7 @@ union Pack {
 };
 
 template <typename T, int V, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeArgs a, int* err) {
+__global__ void __launch_bounds__(kRopeThreads, 5) rope_append_kernel(const RopeArgs a, int* err) {
   pdl_wait();
   pdl_trigger();
   using Raw = typename RawVec<V * (int)sizeof(T)>::type;
@@ -208,58 +217,69 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeArg
   const long long t = (long long)blockIdx.x * (kRopeThreads / nt) + threadIdx.x / nt;
   if (t >= d.tokens) return;
   const int half = d.rot_dim / 2;
-  for (int x = 0; x < d.axes; ++x) {
-    const int pos = __ldg(a.positions + (long long)x * d.tokens + t);
-    if ((unsigned)pos >= (unsigned)d.max_pos) {
-      record_error(err, MDLC_DEVERR_BOUNDS);
-      return;
-    }
-  }
   const int slot = __ldg(a.slots + t);
-  const bool stored = slot >= 0 && slot < d.pages * d.page;
-  if (slot >= 0 && !stored) record_error(err, MDLC_DEVERR_BOUNDS);
+  int pos[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) pos[x] = x < d.axes ? __ldg(a.positions + (long long)x * d.tokens + t) : 0;
   const T* q = static_cast<const T*>(a.q) + t * d.q_stride;
   const T* k = static_cast<const T*>(a.k) + t * d.k_stride;
   const T* v = static_cast<const T*>(a.v) + t * d.v_stride;
   T* qo = a.q_out ? static_cast<T*>(a.q_out) + t * d.out_stride : nullptr;
+  const int hr = d.heads + d.kv_heads, h0 = qo ? 0 : d.heads;  // heads that turn: [h0, hr)
+  auto src_of = [&](int h) { return h < d.heads ? q + (long long)h * d.head_dim : k + (long long)(h - d.heads) * d.head_dim; };
+
+  // the first batch's loads do not wait for the slot, the positions and the angles behind them
+  const int units = half / V;  // per head
+  const int lanes = units ? div_small(nt, a.units) : 0;
+  const int hl = units ? div_small(tl, a.units) : 0, u = tl - hl * units;
+  const int o0 = INTERLEAVED ? 2 * u * V : u * V, o1 = INTERLEAVED ? o0 + V : o0 + half;
+  Pack<T, V> x[kRopeBatch], y[kRopeBatch];
+  auto load_batch = [&](int hb) {
+#pragma unroll
+    for (int j = 0; j < kRopeBatch; ++j) {
+      const int h = hb + j * lanes;
+      if (h < hr) {
+        const T* s = src_of(h);
+        x[j].raw = *reinterpret_cast<const Raw*>(s + o0);
+        y[j].raw = *reinterpret_cast<const Raw*>(s + o1);
+      }
+    }
+  };
+  if (hl < lanes) load_batch(h0 + hl);
+
+  bool known = true;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) known &= (unsigned)pos[i] < (unsigned)d.max_pos;
+  if (!known) {
+    record_error(err, MDLC_DEVERR_BOUNDS);
+    return;
+  }
+  const bool stored = slot >= 0 && slot < d.pages * d.page;
+  if (slot >= 0 && !stored) record_error(err, MDLC_DEVERR_BOUNDS);
   // element offset of (slot, head 0) in a cache, and between its heads
   const long long head_step = (long long)d.page * d.head_dim;
-  const long long at = stored ? (long long)(slot / d.page) * d.kv_heads * head_step + (long long)(slot % d.page) * d.head_dim : 0;
+  const int page_id = a.page_shift >= 0 ? slot >> a.page_shift : slot / d.page;
+  const long long at = stored ? (long long)page_id * d.kv_heads * head_step + (long long)(slot - page_id * d.page) * d.head_dim : 0;
   T* kc = static_cast<T*>(a.k_cache) + at;
   T* vc = static_cast<T*>(a.v_cache) + at;
-  const int hr = d.heads + d.kv_heads;
-  const int h0 = qo ? 0 : d.heads, h1 = stored ? hr : d.heads;  // heads to write
-  auto src_of = [&](int h) { return h < d.heads ? q + (long long)h * d.head_dim : k + (long long)(h - d.heads) * d.head_dim; };
+  const int h1 = stored ? hr : d.heads;  // heads to write
   auto dst_of = [&](int h) { return h < d.heads ? qo + (long long)h * d.head_dim : kc + (h - d.heads) * head_step; };
 
-  const int units = half / V;  // per head
-  const int lanes = units ? nt / units : 0;
-  const int u = units ? tl % units : 0, hl = units ? tl / units : 0;
   if (hl < lanes) {
     float cs[V], sn[V];
-    // axis by axis: pair i belongs to the axis whose section holds it
-    int end = d.section[0], axis = 0;
+    // pair i belongs to the axis whose section holds it
+    const int e0 = d.section[0], e1 = e0 + d.section[1], e2 = e1 + d.section[2];  // sections past `axes` are 0
+    const float2* tab = a.table + u * V;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int pair = u * V + i;
-      while (pair >= end) end += d.section[++axis];
-      const int pos = __ldg(a.positions + (long long)axis * d.tokens + t);
-      const float2 w = __ldg(a.table + (long long)pos * half + pair);
+      const int p = pair < e0 ? pos[0] : (pair < e1 ? pos[1] : (pair < e2 ? pos[2] : pos[3]));
+      const float2 w = __ldg(tab + (long long)p * half + i);
       cs[i] = w.x;
       sn[i] = w.y;
     }
-    const int o0 = INTERLEAVED ? 2 * u * V : u * V, o1 = INTERLEAVED ? o0 + V : o0 + half;
     for (int hb = h0 + hl; hb < h1; hb += lanes * kRopeBatch) {
-      Pack<T, V> x[kRopeBatch], y[kRopeBatch];
-#pragma unroll
-      for (int j = 0; j < kRopeBatch; ++j) {
-        const int h = hb + j * lanes;
-        if (h < h1) {
-          const T* s = src_of(h);
-          x[j].raw = *reinterpret_cast<const Raw*>(s + o0);
-          y[j].raw = *reinterpret_cast<const Raw*>(s + o1);
-        }
-      }
+      if (hb != h0 + hl) load_batch(hb);
 #pragma unroll
       for (int j = 0; j < kRopeBatch; ++j) {
         const int h = hb + j * lanes;
@@ -290,15 +310,17 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(const RopeArg
   }
   // the part of each head that does not turn, and the values
   const int rest = (d.head_dim - d.rot_dim) / V;
-  for (int i = tl; i < (h1 - h0) * rest; i += nt) {
-    const int h = h0 + i / rest, o = d.rot_dim + (i % rest) * V;
-    *reinterpret_cast<Raw*>(dst_of(h) + o) = *reinterpret_cast<const Raw*>(src_of(h) + o);
+  if (rest) {
+    for (int i = tl; i < (h1 - h0) * rest; i += nt) {
+      const int hi = div_small(i, a.rest), h = h0 + hi, o = d.rot_dim + (i - hi * rest) * V;
+      *reinterpret_cast<Raw*>(dst_of(h) + o) = *reinterpret_cast<const Raw*>(src_of(h) + o);
+    }
   }
   if (stored) {
     const int vu = d.head_dim / V;
 #pragma unroll 2
     for (int i = tl; i < d.kv_heads * vu; i += nt) {
-      const int h = i / vu, o = (i % vu) * V;
+      const int h = div_small(i, a.vals), o = (i - h * vu) * V;
       *reinterpret_cast<Raw*>(vc + h * head_step + o) = *reinterpret_cast<const Raw*>(v + (long long)h * d.head_dim + o);
     }
   }
@@ -364,7 +386,9 @@ extern "C" int mdlc_rope_append(mdlc_ctx* ctx, const mdlc_rope_desc* d, const vo
   if ((long long)d->pages * d->page > INT32_MAX)
     return mdlc_set_error(ctx, MDLC_ERR_INVALID, "rope_append: pages * page exceeds 2^31 - 1");
   const long long hw = (long long)d->heads * d->head_dim, kw = (long long)d->kv_heads * d->head_dim;
-  if (hw > INT32_MAX || d->q_stride < hw || d->k_stride < kw || d->v_stride < kw || (q_out && d->out_stride < hw))
+  if ((d->heads + d->kv_heads) * (long long)d->head_dim > 65535)
+    return mdlc_set_error(ctx, MDLC_ERR_UNSUPPORTED, "rope_append: a token of more than 65535 elements");
+  if ( d->q_stride < hw || d->k_stride < kw || d->v_stride < kw || (q_out && d->out_stride < hw))
     return mdlc_set_error(ctx, MDLC_ERR_INVALID, "rope_append: a token stride is smaller than its heads");
   const int esz = d->dtype == MDLC_BF16 ? 2 : 4;
   const uintptr_t addr = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)k_cache | (uintptr_t)v_cache;
@@ -373,11 +397,21 @@ extern "C" int mdlc_rope_append(mdlc_ctx* ctx, const mdlc_rope_desc* d, const vo
   // the widest vector that every pointer, stride and run of pairs allows
   const long long strides = d->q_stride | d->k_stride | d->v_stride | (q_out ? d->out_stride : 0);
   auto fits = [&](int vec) { return (d->rot_dim / 2) % vec == 0 && d->head_dim % vec == 0 && strides % vec == 0 && addr % (vec * esz) == 0; };
-  RopeArgs a = {*d, q, k, v, positions, reinterpret_cast<const float2*>(table), slots, q_out, k_cache, v_cache, 1};
   const int full = 16 / esz;
-  const int vec = fits(full) ? full : (fits(4) ? 4 : 1);
-  // few tokens: a block each, so that the heads are read at once; element by element: 128 units need a block
-  a.warps_per_token = (vec == 1 || d->tokens < 4 * ctx->num_sms) ? kRopeThreads / 32 : 1;
+  const int vec = fits(full) ? full : (fits(4) ? 4 : 1), units = d->rot_dim / 2 / vec;
+  RopeArgs a = {*d, q, k, v, positions, reinterpret_cast<const float2*>(table), slots, q_out, k_cache, v_cache};
+  for (int i = d->axes; i < 4; ++i) a.d.section[i] = 0;
+  a.units = small_div(max(1, units));
+  a.rest = small_div(max(1, (d->head_dim - d->rot_dim) / vec));
+  a.vals = small_div(d->head_dim / vec);
+  a.page_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (d->page == 1 << i) a.page_shift = i;
+  // Warps of a token: enough for one batch of loads per thread to hold all of its heads; few tokens, or element by element
+  // (128 units): a block
+  a.warps_per_token = 1;
+  while (a.warps_per_token < kRopeThreads / 32 && units && a.warps_per_token * 32 / units * kRopeBatch < d->heads + d->kv_heads) a.warps_per_token *= 2;
+  if (vec == 1 || d->tokens < 4 * ctx->num_sms) a.warps_per_token = kRopeThreads / 32;
   cudaError_t e;
   if (esz == 2)
     e = vec == 8 ? launch_rope<__nv_bfloat16, 8>(ctx, a) : (vec == 4 ? launch_rope<__nv_bfloat16, 4>(ctx, a) : launch_rope<__nv_bfloat16, 1>(ctx, a));
