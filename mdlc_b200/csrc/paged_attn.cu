@@ -63,11 +63,12 @@ MDLC_DEV void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint3
 // high part (a tf32 value) and the exact rest of an fp32 number
 MDLC_DEV uint32_t tf_hi(uint32_t x) { return x & 0xffffe000u; }
 MDLC_DEV uint32_t tf_lo(uint32_t x) { return __float_as_uint(__uint_as_float(x) - __uint_as_float(tf_hi(x))); }
-// c += a b of fp32 operands in three tf32 products, the small ones first
-MDLC_DEV void mma_3tf32(float (&c)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], uint32_t b0, uint32_t b1) {
-  mma_tf32(c, lo, tf_hi(b0), tf_hi(b1));
-  mma_tf32(c, hi, tf_lo(b0), tf_lo(b1));
+// a b of fp32 operands in three tf32 products: c takes the large one, r the two small ones (sums of their own: shorter chains
+// of dependent products, and the truncation of one does not cut the other)
+MDLC_DEV void mma_3tf32(float (&c)[4], float (&r)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], uint32_t b0, uint32_t b1) {
   mma_tf32(c, hi, tf_hi(b0), tf_hi(b1));
+  mma_tf32(r, lo, tf_hi(b0), tf_hi(b1));
+  mma_tf32(r, hi, tf_lo(b0), tf_lo(b1));
 }
 
 MDLC_DEV void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -197,6 +198,8 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
 
     // scores
     float s[BT / 8][4] = {};
+    constexpr int ST = kBf16 ? 1 : BT / 8;
+    float s_odd[ST][4] = {}, s_low[ST][4] = {};  // fp32: odd steps' products and the small ones
     {
       const int mi = lane >> 3, r = lane & 7;
       const int key = (mi >> 1) * 8 + r;
@@ -216,10 +219,16 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
               hi[i] = tf_hi(qa[ks][i]);
               lo[i] = tf_lo(qa[ks][i]);
             }
-            mma_3tf32(s[nt], hi, lo, kb[0], kb[1]);
-            mma_3tf32(s[nt + 1], hi, lo, kb[2], kb[3]);
+            mma_3tf32(ks & 1 ? s_odd[nt] : s[nt], s_low[nt], hi, lo, kb[0], kb[1]);
+            mma_3tf32(ks & 1 ? s_odd[nt + 1] : s[nt + 1], s_low[nt + 1], hi, lo, kb[2], kb[3]);
           }
         }
+      if constexpr (!kBf16) {
+#pragma unroll
+        for (int nt = 0; nt < BT / 8; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[nt][i] += s_odd[nt][i] + s_low[nt][i];
+      }
     }
     // mask, running maximum. A block that every row sees whole (all but the span's ends) needs no mask.
     const bool open = valid == (BT == 32 ? 0xffffffffu : (1u << BT) - 1u) && base + BT - 1 <= shift + r0 / a.group &&
@@ -254,7 +263,7 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
     }
     // the tensor cores truncate the running sum at every addition, an error that grows with the number of
     // keys: for fp32 each block is summed from zero and added with a rounded addition (over 1700 keys
-    // the error falls from 1.1e-5 to the plain form's; bf16 outputs do not show it)
+    // the error falls from 1.1e-5 to F32_ERR; bf16 outputs do not show it)
 #pragma unroll
     for (int nt = 0; nt < BT / 8; ++nt)
 #pragma unroll
@@ -295,15 +304,15 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
 #pragma unroll
       for (int nd = 0; nd < HDP / 8; ++nd) {
         const int c = nd * 2 + (g >> 2);
-        float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        float add[2][4] = {}, low[4] = {};
 #pragma unroll
         for (int kt = 0; kt < BT / 8; ++kt) {
           const uint32_t b0 = lds32(vs_addr + (kt * 8 + k0) * PITCH + ((c ^ k0) << 4) + (g & 3) * 4);
           const uint32_t b1 = lds32(vs_addr + (kt * 8 + k1) * PITCH + ((c ^ k1) << 4) + (g & 3) * 4);
-          mma_3tf32(add, hi[kt], lo[kt], b0, b1);
+          mma_3tf32(add[kt & 1], low, hi[kt], lo[kt], b0, b1);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[nd][i] += add[i];
+        for (int i = 0; i < 4; ++i) o[nd][i] += (add[0][i] + add[1][i]) + low[i];
       }
     }
     stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -980,7 +989,7 @@ cudaError_t run_attn(mdlc_ctx* ctx, AttnArgs& a) {
   }
   if (e != cudaSuccess || c.splits == 1) return e;
   mdlc_note_launch(ctx);
-  return launch_pdl(attn_chunk_join_kernel<T, HDP>, dim3(c.tiles, a.d.kv_heads, c.rows / 64), dim3(kJoinThreads), 0, ctx->stream, a, c.rows,
+  return launch_pdl(attn_chunk_join_kernel<T, HDP>, dim3(c.tiles, a.d.kv_heads, c.rows / 16), dim3(kJoinThreads), 0, ctx->stream, a, c.rows,
                     c.tc ? kTcKeys : block_keys<T, HDP>());
 }
 
