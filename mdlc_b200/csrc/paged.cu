@@ -38,7 +38,19 @@ MDLC_DEV Sums warp_scan(Sums v, int lane) {
   return v;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page_desc d, const PlanPtrs p, int* err) {
+// division by the page size: a shift where it is a power of two (64-bit divisions were most of a small plan's time)
+struct PageDiv {
+  uint32_t page;
+  int shift;  // -1: not a power of two
+};
+MDLC_DEV uint32_t page_index(uint32_t tok, const PageDiv& d) { return d.shift >= 0 ? tok >> d.shift : tok / d.page; }
+// pages of tok tokens (two int32 lengths' sum fits 32 bits unsigned)
+MDLC_DEV uint32_t pages_of(uint32_t tok, const PageDiv& d) {
+  const uint32_t n = page_index(tok, d);
+  return n + (n * d.page != tok);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page_desc d, const PlanPtrs p, const PageDiv pd) {
   pdl_wait();
   pdl_trigger();
   extern __shared__ int32_t plan_smem[];
@@ -56,12 +68,11 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page
   const int per = (d.batch + kPlanThreads - 1) / kPlanThreads;
   const int b0 = min(tid * per, d.batch), b1 = min(b0 + per, d.batch);
   Sums mine = {0, 0};
-  auto pages_of = [&](long long tok) { return (tok + d.page - 1) / d.page; };
   // pages that request b takes (0 where it does not fit its table row), and whether it fits
   auto ask = [&](int c, int n, bool* fits) {
-    const long long need = pages_of((long long)c + n);
-    *fits = need <= d.table_stride;
-    return *fits ? need - pages_of(c) : 0ll;
+    const uint32_t need = pages_of((uint32_t)c + (uint32_t)n, pd);
+    *fits = need <= (uint32_t)d.table_stride;
+    return *fits ? need - pages_of(c, pd) : 0u;
   };
   for (int b = b0; b < b1; ++b) {
     const int c = max(0, __ldg(p.cached + b)), n = max(0, __ldg(p.fresh + b));
@@ -88,7 +99,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page
   for (int b = b0; b < b1; ++b) {
     const int c = max(0, __ldg(p.cached + b)), n = max(0, __ldg(p.fresh + b));
     bool fits;
-    const long long take = ask(c, n, &fits);
+    const uint32_t take = ask(c, n, &fits);
     const bool ok = fits && (take == 0 || run.pages + take <= n_free);
     starts[b] = (int32_t)min(run.tokens, (long long)d.tokens);
     held_tok[b] = c;
@@ -121,7 +132,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page
   for (int b = blockIdx.x * (kPlanThreads / 32) + warp; b < d.batch; b += nwarps) {
     if (first[b] < 0) continue;
     const int c = held_tok[b];
-    const int held = (int)pages_of(c), take = (int)(pages_of((long long)c + max(0, __ldg(p.fresh + b))) - held);
+    const int held = (int)pages_of(c, pd), take = (int)pages_of((uint32_t)c + (uint32_t)max(0, __ldg(p.fresh + b)), pd) - held;
     for (int j = lane; j < take; j += 32)
       p.table[(long long)b * d.table_stride + held + j] = __ldg(p.free_list + first[b] + j);
   }
@@ -138,11 +149,11 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page
       const int c = held_tok[lo];
       pos = c + (t - starts[lo]);
       if (first[lo] >= 0) {
-        const int at = pos / d.page, held = (int)pages_of(c);
+        const int at = (int)page_index(pos, pd), held = (int)pages_of(c, pd);
         // a page taken by this call comes from the free list itself: its table entry may not be written yet
         const int id = at < held ? __ldg(p.table + (long long)lo * d.table_stride + at)
                                  : __ldg(p.free_list + first[lo] + (at - held));
-        if (id >= 0) slot = id * d.page + pos % d.page;
+        if (id >= 0) slot = id * d.page + (pos - at * d.page);
       }
     }
     p.slots[t] = slot;
@@ -361,7 +372,10 @@ extern "C" int mdlc_page_plan(mdlc_ctx* ctx, const mdlc_page_desc* d, const int3
   // two tokens per thread; the scan is repeated in each block, so no more blocks than SMs
   const int blocks = (int)min((long long)ctx->num_sms, ((long long)d->tokens + 2 * kPlanThreads - 1) / (2 * kPlanThreads));
   const PlanPtrs p = {cached_lens, new_lens, free_list, free_count, block_table, q_starts, kv_lens, slots, positions, status};
-  const cudaError_t e = launch_pdl(page_plan_kernel, dim3(blocks), dim3(kPlanThreads), smem, ctx->stream, *d, p, ctx->d_err);
+  PageDiv pd = {(uint32_t)d->page, -1};
+  for (int i = 0; i <= 10; ++i)
+    if (d->page == 1 << i) pd.shift = i;
+  const cudaError_t e = launch_pdl(page_plan_kernel, dim3(blocks), dim3(kPlanThreads), smem, ctx->stream, *d, p, pd);
   mdlc_note_launch(ctx);
   return mdlc_cuda_status(ctx, e, "page_plan launch");
 }

@@ -9,10 +9,10 @@
 //     after one shift. (As bf16 operands they took 11 operations, two of them per pair of
 //     codes, and the kernel was bound by the integer pipe: 79 us at one row of 65536 x 8192 where this
 //     one takes 56 us, 4.9 TB/s.)
-//   * x is written once per block as fixed-point numbers of 23 bits, a power of two per row and
-//     group of columns (the largest magnitude just below 2^22), cut into three balanced signed
-//     base-256 digits, each a column of the 8-column operand. The error is at most 2^-23 of the group's largest |x|:
-//     what an fp32 product with that element would round.
+//   * x is written once as fixed-point numbers of 23 bits, a power of two per row and 128 columns
+//     (the largest magnitude just below 2^22), cut into three balanced signed base-256 digits, each a
+//     column of the 8-column operand. The error is at most 2^-23 of the largest |x| of those columns: what an fp32 product
+//     with that element would round.
 //   * a group's int32 sums (below 2^21) start from the bits of 1.5 x 2^23, so they are fp32 numbers as they
 //     stand; they are scaled and added to the row's fp32 sum once per group. A zero point z other
 //     than 8 adds (8 - z) times the digits' sum.
@@ -48,6 +48,7 @@ struct W4Args {
   int step_bytes;       // x of one step, see w4_step_bytes
   int span, buffers;    // steps in shared memory at a time, and their buffers
   const uint8_t* ready; // x as digits, [chunk][step], or null: the block makes them itself
+  bool ready_wanted;
   int* err;
 };
 
@@ -85,21 +86,22 @@ MDLC_DEV void quad_transpose(uint32_t (&w)[4], int t) {
 
 // x as digits, one 128-column step of k after the other, each: 16 units of 8 columns x pitch columns x 8 bytes (the digits of
 // columns 0, 2, 4, 6 and 1, 3, 5, 7; units and columns permuted so that the four units a warp reads at once,
-// 4 apart or adjacent, lie in different banks); per group its columns' weights / 256 (fp32); per group the digits' sums (fp32)
+// 4 apart or adjacent, lie in different banks); the columns' weights / 256 (fp32); per group of the weights the digits' sums (fp32)
 MDLC_DEV int x_place(int unit, int col, int pitch) {
   const int v = unit ^ ((unit >> 2) & 3);
   return v * pitch + (pitch == 4 ? col : col ^ ((v & 2) << 1));
 }
-__host__ __device__ inline int w4_step_bytes(int pitch, int group) { return pitch * (128 + 128 / group * 8); }
+__host__ __device__ inline int w4_step_bytes(int pitch, int group) { return pitch * (128 + 4 + 128 / group * 4); }
 
-// Eight columns of an x row as digits, by one lane; the lanes of a group (neighbours) share an exponent. u: unit; dst: the
-// step that holds it. Every lane of the warp calls this; `ok`: the unit exists.
-MDLC_DEV void x_digits(const float (&f)[8], int u, int col0, int log_group, int pitch, uint8_t* dst, bool ok) {
-  const int per = (1 << log_group) / 8;
+// Eight columns of an x row as digits, by one lane; the 16 lanes of a step (neighbours) share an exponent. u: unit; dst: the
+// step that holds it. Every lane of the warp calls this; `ok`: the unit is one of a step's (past k: zeros).
+MDLC_DEV void x_digits(const float (&f)[8], int u, int col0, int group, int pitch, uint8_t* dst, bool ok) {
+  const int per = group / 8;
   uint32_t top = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
-  for (int o = 1; o < per; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+  for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
   // |x| < 2^(ex - 126); below 2^-96 the digits get shorter
   const bool finite = top < 0x7f800000u;
   const int ex = max((int)(top >> 23), 30);
@@ -117,7 +119,7 @@ MDLC_DEV void x_digits(const float (&f)[8], int u, int col0, int log_group, int 
     down = __uint_as_float(top);
   }
   uint2* units = reinterpret_cast<uint2*>(dst);
-  float* xf = reinterpret_cast<float*>(dst + 128 * pitch) + ((u & 15) * 8 >> log_group) * pitch;
+  float* xf = reinterpret_cast<float*>(dst + 128 * pitch);
 #pragma unroll
   for (int p = 0; p < 3; ++p) {
     const uint32_t two = p | ((4 + p) << 4);
@@ -127,10 +129,8 @@ MDLC_DEV void x_digits(const float (&f)[8], int u, int col0, int log_group, int 
     if (ok) units[x_place(u & 15, col0 + p, pitch)] = b;
     int sum = __dp4a((int)b.x, 0x01010101, __dp4a((int)b.y, 0x01010101, 0));
     for (int o = 1; o < per; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (ok && (u & (per - 1)) == 0) {
-      xf[col0 + p] = p == 0 ? down : (finite ? down * (p == 1 ? 256.0f : 65536.0f) : 0.0f);
-      xf[(128 >> log_group) * pitch + col0 + p] = (float)sum;
-    }
+    if (ok && (u & 15) == 0) xf[col0 + p] = p == 0 ? down : (finite ? down * (p == 1 ? 256.0f : 65536.0f) : 0.0f);
+    if (ok && (u & (per - 1)) == 0) xf[(1 + (u & 15) / per) * pitch + col0 + p] = (float)sum;
   }
 }
 MDLC_DEV void x_load(const W4Args& a, int row, int u, bool ok, float (&f)[8]) {
@@ -159,12 +159,11 @@ __global__ void __launch_bounds__(128) w4_digits_kernel(const W4Args a, uint8_t*
   pdl_trigger();
   const int units = a.d.k / 8, lane = threadIdx.x & 31, steps = (a.d.k + 127) / 128;
   const int u = (blockIdx.x * 4 + (threadIdx.x >> 5)) * 32 + lane, row = blockIdx.y;
-  const bool ok = u < units;
   float f[8];
-  x_load(a, row, u, ok, f);
+  x_load(a, row, u, u < units, f);
   const int chunk = row / a.rows_per_chunk;
   uint8_t* dst = ready + ((long long)chunk * steps + min(u / 16, steps - 1)) * a.step_bytes;
-  x_digits(f, u, 3 * (row - chunk * a.rows_per_chunk), 31 - __clz(a.d.group), a.pitch, dst, ok);
+  x_digits(f, u, 3 * (row - chunk * a.rows_per_chunk), a.d.group, a.pitch, dst, u < 16 * steps);
 }
 
 // a run of bytes (16-byte aligned, a multiple of 16) into shared memory, completing on an mbarrier
@@ -179,11 +178,11 @@ MDLC_DEV float2 add2(const float2 a, const float2 b) {
   return f2_from(r);
 }
 
-// NT: 8-column tiles; R: 16-row tiles; G128: groups of 128 columns; ZEROS: zero points given
+// NT: 8-column tiles; R: 16-row tiles; GROUP: columns of a group; ZEROS: zero points given
 template <int NT, int R>
 constexpr int w4_min_blocks() { return NT * R <= 3 ? 2 : 1; }
 
-template <int NT, int R, bool G128, bool ZEROS>
+template <int NT, int R, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4_kernel(const W4Args a) {
   pdl_wait();
   pdl_trigger();
@@ -198,7 +197,8 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
   __shared__ __align__(8) uint64_t x_bar[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int m0 = blockIdx.y * a.rows_per_chunk, mc = min(a.rows_per_chunk, d.m - m0);
-  const int log_group = 31 - __clz(d.group), groups = d.k >> log_group, half = d.k / 2;
+  constexpr bool G128 = GROUP == 128;
+  const int groups = d.k / GROUP, half = d.k / 2;
   const int steps = (d.k + 127) / 128, tiles = (d.n + 16 * R - 1) / (16 * R);
 
   // This block's tiles are blockIdx.x, + gridDim.x, ...; the warp's steps of all of them form one line, along which
@@ -233,8 +233,8 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
       enter();
     }
   };
-  // scales and zero points of a step, one set per 32 columns (G128: one for all)
-  constexpr int SETS = G128 ? 1 : 4;
+  // scales and zero points of a step's groups (past k: the last group's, for columns whose digits are 0)
+  constexpr int SETS = 128 / GROUP;
   uint32_t sc[SETS][R][2] = {}, sc_next[SETS][R][2] = {}, zr[SETS][R][2] = {}, zr_next[SETS][R][2] = {};
   int s_tile = blockIdx.x, s_step = warp;
   const uint16_t* sp[R][2];
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
     if (s_tile < tiles && s_step < steps) {
 #pragma unroll
       for (int i = 0; i < SETS; ++i) {
-        const uint32_t grp = G128 ? s_step : min((s_step * 128 + 32 * i) >> log_group, groups - 1);
+        const uint32_t grp = G128 ? s_step : min(s_step * SETS + i, groups - 1);
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -300,13 +300,13 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
     }
   } else {
     const int units = d.k / 8;
-    for (int u0 = warp * 32; u0 < units; u0 += 2 * kW4Warps * 32) {  // two loads at a time
+    for (int u0 = warp * 32; u0 < 16 * steps; u0 += 2 * kW4Warps * 32) {  // two loads at a time
       const int u1 = u0 + kW4Warps * 32 + lane, ua = u0 + lane;
       float fa[8], fb[8];
       x_load(a, m0, ua, ua < units, fa);
       x_load(a, m0, u1, u1 < units, fb);
-      x_digits(fa, ua, 0, log_group, pitch, xs + min(ua / 16, steps - 1) * a.step_bytes, ua < units);
-      x_digits(fb, u1, 0, log_group, pitch, xs + min(u1 / 16, steps - 1) * a.step_bytes, u1 < units);
+      x_digits(fa, ua, 0, GROUP, pitch, xs + min(ua / 16, steps - 1) * a.step_bytes, ua < 16 * steps);
+      x_digits(fb, u1, 0, GROUP, pitch, xs + min(u1 / 16, steps - 1) * a.step_bytes, u1 < 16 * steps);
     }
   }
   __syncthreads();
@@ -351,11 +351,11 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
         slot = (slot + 1) % kW4Depth;
         const uint8_t* x_at = buf + (s - s0) * a.step_bytes;
         uint32_t acc[R][NT][4];
+        float2 part[R][NT][2] = {};  // the step's sums of scaled groups
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           // word i holds columns 32 t + 8 i of this step (G128) or, after the exchange, 32 i + 8 t
-          const bool in = G128 || s * 128 + 32 * i < d.k;  // the last step may end early, at a multiple of 32
-          const bool first = i == 0 || (!G128 && ((32 * i) & (d.group - 1)) == 0);
+          const bool first = G128 ? i == 0 : 32 * i % GROUP == 0;
           if (first) {
 #pragma unroll
             for (int r = 0; r < R; ++r)
@@ -367,10 +367,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
           // columns without an x row read what lies there (a single row's are read twice): their sums are not used
           uint2 b[NT];
 #pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            b[j] = make_uint2(0, 0);
-            if (in) b[j] = *reinterpret_cast<const uint2*>(x_at + x_off[i] + 64 * j);
-          }
+          for (int j = 0; j < NT; ++j) b[j] = *reinterpret_cast<const uint2*>(x_at + x_off[i] + 64 * j);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const uint32_t a0 = high_codes(w[r][0][i] << 4), a1 = high_codes(w[r][1][i] << 4);
@@ -378,25 +375,33 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
 #pragma unroll
             for (int j = 0; j < NT; ++j) mma_s8(acc[r][j], a0, a1, a2, a3, b[j].x, b[j].y);
           }
-          const bool last = G128 ? i == 3 : ((32 * (i + 1)) & (d.group - 1)) == 0;
-          if (last && in) {
-            const int set = G128 ? 0 : i;
-            const uint8_t* fp = x_at + f_off + (G128 ? 0 : (32 * i >> log_group) * pitch * 4);
+          const bool last = G128 ? i == 3 : 32 * (i + 1) % GROUP == 0;
+          if (last) {
+            const int set = G128 ? 0 : 32 * i / GROUP;
+            const uint8_t* dp = x_at + f_off + (1 + set) * pitch * 4;
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              const float2 fx = *reinterpret_cast<const float2*>(fp + 32 * j);
               float2 dx = splat2(0.0f);
-              if (ZEROS) dx = *reinterpret_cast<const float2*>(fp + (128 >> log_group) * pitch * 4 + 32 * j);
+              if (ZEROS) dx = *reinterpret_cast<const float2*>(dp + 32 * j);
 #pragma unroll
               for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                  float2 f = add2(make_float2(__uint_as_float(acc[r][j][2 * h]), __uint_as_float(acc[r][j][2 * h + 1])), splat2(-12582912.0f));
+                  float2 f = splat2(-12582912.0f);
                   if (ZEROS) f = fma2(splat2(__uint_as_float(kMagic + 128u - 16u * (zr[set][r][h] & 15u)) - 12582912.0f), dx, f);
-                  out[r][j][h] = fma2(fmul2(splat2(__uint_as_float(sc[set][r][h] << 16)), fx), f, out[r][j][h]);
+                  f = add2(make_float2(__uint_as_float(acc[r][j][2 * h]), __uint_as_float(acc[r][j][2 * h + 1])), f);
+                  part[r][j][h] = fma2(splat2(__uint_as_float(sc[set][r][h] << 16)), f, part[r][j][h]);
                 }
             }
           }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const float2 fx = *reinterpret_cast<const float2*>(x_at + f_off + 32 * j);
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) out[r][j][h] = fma2(fx, part[r][j][h], out[r][j][h]);
         }
       }
     }
@@ -438,18 +443,28 @@ template <int NT, int R>
 W4Plan w4_plan(const W4Args& a, int num_sms) {
   W4Plan p = {};
   const int steps = (a.d.k + 127) / 128, rest = kW4Warps * 32 * kW4Depth * R * 2 * 16 + kW4Warps * 16 * R * (8 * NT + 2) * 4;
-  const int room = 226 * 1024 - rest;
-  if ((long long)steps * a.step_bytes <= room) {
-    p.span = steps;
-    p.buffers = 1;
-  } else {
-    p.span = room / 2 / a.step_bytes / kW4Warps * kW4Warps;  // a whole number of the warps' rounds
-    p.buffers = 2;
-  }
-  p.smem = rest + p.buffers * p.span * a.step_bytes;
-  p.blocks = num_sms * (w4_min_blocks<NT, R>() == 2 && 2 * (p.smem + 1024) <= 227 * 1024 ? 2 : 1);
   p.tiles = (a.d.n + 16 * R - 1) / (16 * R);
-  return p;
+  // per_sm blocks on an SM: all of x where it fits beside the rest, else two buffers of a whole number of the warps' rounds
+  auto fit = [&](int per_sm) {
+    W4Plan q = p;
+    const int room = 226 * 1024 / per_sm - 1024 - rest;
+    if ((long long)steps * a.step_bytes <= room) {
+      q.span = steps;
+      q.buffers = 1;
+    } else {
+      q.span = a.ready_wanted ? max(0, room) / 2 / a.step_bytes / kW4Warps * kW4Warps : 0;
+      q.buffers = 2;
+    }
+    q.smem = rest + q.buffers * q.span * a.step_bytes;
+    q.blocks = num_sms * per_sm;
+    return q;
+  };
+  const W4Plan one = fit(1);
+  if (w4_min_blocks<NT, R>() < 2) return one;
+  const W4Plan two = fit(2);
+  // two buffers read x again for every tile: worth two blocks on an SM only where that is little beside the weights
+  const bool little = two.buffers == 1 || (double)p.tiles * steps * a.step_bytes <= 0.5 * a.d.n * a.d.k;
+  return two.span && (!one.span || (little && two.rounds() < one.rounds())) ? two : one;
 }
 
 template <int NT, int R>
@@ -457,13 +472,14 @@ cudaError_t launch_w4(mdlc_ctx* ctx, W4Args& a, const W4Plan& p) {
   a.span = p.span;
   a.buffers = p.buffers;
   const dim3 grid(min(p.tiles, p.blocks), (a.d.m + a.rows_per_chunk - 1) / a.rows_per_chunk);
-  static SmemLimit seen[4];
+  static SmemLimit seen[6];
   auto go = [&](int which, auto* kern) {
     const cudaError_t e = allow_smem(seen[which], ctx->device, kern, p.smem);
     return e != cudaSuccess ? e : launch_pdl(kern, grid, dim3(kW4Warps * 32), p.smem, ctx->stream, a);
   };
-  if (a.d.group == 128) return a.zeros ? go(0, gemv_w4_kernel<NT, R, true, true>) : go(1, gemv_w4_kernel<NT, R, true, false>);
-  return a.zeros ? go(2, gemv_w4_kernel<NT, R, false, true>) : go(3, gemv_w4_kernel<NT, R, false, false>);
+  if (a.d.group == 128) return a.zeros ? go(0, gemv_w4_kernel<NT, R, 128, true>) : go(1, gemv_w4_kernel<NT, R, 128, false>);
+  if (a.d.group == 64) return a.zeros ? go(2, gemv_w4_kernel<NT, R, 64, true>) : go(3, gemv_w4_kernel<NT, R, 64, false>);
+  return a.zeros ? go(4, gemv_w4_kernel<NT, R, 32, true>) : go(5, gemv_w4_kernel<NT, R, 32, false>);
 }
 
 template <int NT>
@@ -472,7 +488,7 @@ cudaError_t launch_w4_cols(mdlc_ctx* ctx, W4Args& a) {
   a.pitch = a.d.m == 1 ? 4 : 8 * NT;
   a.step_bytes = w4_step_bytes(a.pitch, a.d.group);
   const long long steps = ((long long)a.d.k + 127) / 128;
-  const bool ready = a.d.m > 1 || steps * a.step_bytes > kW4OwnX;
+  const bool ready = a.ready_wanted = a.d.m > 1 || steps * a.step_bytes > kW4OwnX;
   // several rows: one kernel makes the digits for all blocks, as many chunks of rows at a time as the context's workspace holds
   const long long fit = (long long)kSplitWsBytes / (steps * a.step_bytes);
   if (ready && fit == 0) return cudaErrorNotSupported;
@@ -501,7 +517,8 @@ cudaError_t launch_w4_cols(mdlc_ctx* ctx, W4Args& a) {
 }
 
 cudaError_t launch_w4_rows(mdlc_ctx* ctx, W4Args& a) {
-  // three columns per row, up to 16 rows in six column tiles (their products then take as long as the weights' bytes)
+  // Three columns per row, up to 16 rows in six column tiles at once. (Fewer tiles at once would let all of x stay in shared memory, but
+  // read the weights again: 16 rows of 14336 x 4096 in six tiles 40 us, in three, twice, 53 us.)
   const int need = (int)min(6ll, (3ll * a.d.m + 7) / 8), nt = need == 5 ? 6 : need;
   switch (nt) {
     case 1: return launch_w4_cols<1>(ctx, a);
@@ -532,7 +549,7 @@ extern "C" int mdlc_gemv_w4(mdlc_ctx* ctx, const mdlc_w4_desc* d, const void* x,
     return mdlc_set_error(ctx, MDLC_ERR_INVALID, "gemv_w4: misaligned pointer");
   if (d->m > 65535) return mdlc_set_error(ctx, MDLC_ERR_UNSUPPORTED, "gemv_w4: %d rows (at most 65535)", d->m);
   cudaSetDevice(ctx->device);
-  W4Args a = {*d, x, codes, static_cast<const uint16_t*>(scales), zeros, bias, y, 0, 0, 0, 0, 0, nullptr, ctx->d_err};
+  W4Args a = {*d, x, codes, static_cast<const uint16_t*>(scales), zeros, bias, y, 0, 0, 0, 0, 0, nullptr, false, ctx->d_err};
   const cudaError_t e = launch_w4_rows(ctx, a);
   if (e == cudaErrorNotSupported) return mdlc_set_error(ctx, MDLC_ERR_UNSUPPORTED, "gemv_w4: k = %d does not fit the workspace", d->k);
   return mdlc_cuda_status(ctx, e, "gemv_w4 launch");
