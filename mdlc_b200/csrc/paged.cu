@@ -1,8 +1,7 @@
 // Bookkeeping of a paged key / value cache: mdlc_page_plan (block tables, slot
 // maps and positions from request lengths) and mdlc_rope_append (rotary
 // positions on queries and keys, keys and values written to their slots).
-#include "common.cuh"
-#include "runtime.h"
+#include "paged_attn.cuh"
 
 namespace mdlc {
 namespace {
@@ -169,13 +168,6 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page
 // batch precede its stores, and no thread reads what another writes).
 constexpr int kRopeThreads = 128;
 constexpr int kRopeBatch = 4;
-
-// n / d for 0 <= n < 65536 and 1 <= d <= 65536 as a product: a runtime division costs some 20 instructions
-struct SmallDiv {
-  uint32_t d, m;  // m = floor((2^32 - 1) / d) + 1
-};
-SmallDiv small_div(int d) { return {(uint32_t)d, 0xffffffffu / (uint32_t)d + 1u}; }
-MDLC_DEV int div_small(int n, const SmallDiv& s) { return s.m ? (int)__umulhi((uint32_t)n, s.m) : n; }  // m wraps to 0 for d = 1
 
 struct RopeArgs {
   mdlc_rope_desc d;

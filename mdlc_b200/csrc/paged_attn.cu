@@ -811,16 +811,16 @@ __global__ void __launch_bounds__(kAttnThreads) attn_chunk_kernel(const AttnArgs
   __shared__ uint32_t valid_s[K::WN][kStages];
   __shared__ long long warp_sums[kAttnThreads / 32];
   __shared__ Place place_s;
-  pdl_wait();
-  pdl_trigger();
+  chunk_begin(a);
   Tile t;
-  if (!find_tile(a, blockIdx.x, K::ROWS, warp_sums, &place_s, &t)) return;
+  if (!find_tile(a, blockIdx.x, K::ROWS, warp_sums, &place_s, &t)) return chunk_end(a);
   const Span sp = span_of(a, t.rq, t.r0 / a.group, (min(t.r0 + K::ROWS, t.rows) - 1) / a.group, K::BT);
   const int ns = splits_of(a, sp.n, kLeastKeys / K::BT), z = blockIdx.z;
   if (z >= ns) return;
   attn_piece<T, HDP, 4>(a, attn_smem, valid_s, err, t.b, t.rq, blockIdx.y, t.r0, sp, (int)((long long)z * sp.n / ns),
                         (int)((long long)(z + 1) * sp.n / ns), ns == 1,
                         ((long long)blockIdx.x * a.d.kv_heads + blockIdx.y) * a.splits + z);
+  chunk_end(a);
 }
 
 // Adds the shares of a chunk tile, in order. A warp per row.
@@ -897,20 +897,22 @@ Chunk chunk_of(const mdlc_attn_desc& d) {
   return c;
 }
 
+// partial sums, maxima and sums of split mode's slots, then chunk mode's (the two run side by side)
 struct Layout {
-  size_t part_o, part_m, part_l, total;
+  size_t o[2], m[2], l[2], total;
 };
 Layout layout_of(const mdlc_attn_desc& d) {
-  const size_t slots = (size_t)d.batch * d.kv_heads + kMaxBlocks;
-  size_t rows = slots * 16 * split_groups(d);
   const Chunk c = chunk_of(d);
-  // the two modes run one after the other and share the space
-  if (c.used && c.splits > 1) rows = max(rows, (size_t)c.tiles * d.kv_heads * c.splits * c.rows);
-  Layout l;
-  l.part_o = 0;
-  l.part_m = align256(rows * padded_dim(d.head_dim) * 4);
-  l.part_l = l.part_m + align256(rows * 4);
-  l.total = l.part_l + align256(rows * 4);
+  const size_t rows[2] = {((size_t)d.batch * d.kv_heads + kMaxBlocks) * 16 * split_groups(d),
+                          c.used && c.splits > 1 ? (size_t)c.tiles * d.kv_heads * c.splits * c.rows : 0};
+  Layout l = {};
+  for (int i = 0; i < 2; ++i) {
+    l.o[i] = l.total;
+    l.m[i] = l.o[i] + align256(rows[i] * padded_dim(d.head_dim) * 4);
+    l.l[i] = l.m[i] + align256(rows[i] * 4);
+    l.total = l.l[i] + align256(rows[i] * 4);
+  }
+  l.total = max(l.total, (size_t)256);
   return l;
 }
 
@@ -960,24 +962,25 @@ cudaError_t run_narrow(mdlc_ctx* ctx, const AttnArgs& a) {
 bool narrow_fits(const mdlc_attn_desc& d) { return d.dtype == MDLC_BF16 && d.page >= 8 && (d.page & (d.page - 1)) == 0; }
 
 template <typename T, int HDP>
-cudaError_t run_attn(mdlc_ctx* ctx, AttnArgs& a) {
+cudaError_t run_attn(mdlc_ctx* ctx, AttnArgs& sa, AttnArgs& a) {  // split mode's and chunk mode's arguments
   const int wm = split_groups(a.d);
   cudaError_t e = cudaSuccess;
   if (wm == 1 && narrow_fits(a.d)) {
     // requests of up to 8 rows in one column tile; with more than 8 heads per key head, or several tokens, two
     const bool one = a.group <= 8 && ((long long)a.d.max_q * a.group <= 8 || (long long)a.d.max_q * a.group > 16);
-    if (one) a.split_rows = 8;
-    e = one ? run_narrow<HDP, 1>(ctx, a) : run_narrow<HDP, 2>(ctx, a);
+    if (one) sa.split_rows = a.split_rows = 8;
+    e = one ? run_narrow<HDP, 1>(ctx, sa) : run_narrow<HDP, 2>(ctx, sa);
   } else if (wm == 1) {
-    e = run_split<T, HDP, 1>(ctx, a);
+    e = run_split<T, HDP, 1>(ctx, sa);
   } else if (wm == 2) {
-    e = run_split<T, HDP, 2>(ctx, a);
+    e = run_split<T, HDP, 2>(ctx, sa);
   } else if (wm == 4) {
-    e = run_split<T, HDP, 4>(ctx, a);
+    e = run_split<T, HDP, 4>(ctx, sa);
   }
   const Chunk c = chunk_of(a.d);
   if (e != cudaSuccess || !c.used) return e;
   a.splits = c.splits;
+  a.beside = wm > 0;
   const dim3 grid(c.tiles, a.d.kv_heads, c.splits);
   mdlc_note_launch(ctx);
   if (c.tc) {
@@ -1027,17 +1030,24 @@ extern "C" int mdlc_paged_attn(mdlc_ctx* ctx, const mdlc_attn_desc* desc, const 
   a.out = out;
   a.lse = lse;
   a.group = desc->heads / desc->kv_heads;
+  a.group_div = small_div(a.group);
   a.split_rows = 16 * split_groups(*desc);
   a.scale_log2 = desc->scale * 1.4426950408889634f;
   const Layout l = layout_of(*desc);
   char* ws = static_cast<char*>(workspace);
-  a.part_o = reinterpret_cast<float*>(ws + l.part_o);
-  a.part_m = reinterpret_cast<float*>(ws + l.part_m);
-  a.part_l = reinterpret_cast<float*>(ws + l.part_l);
+  auto place = [&](int mode) {
+    a.part_o = reinterpret_cast<float*>(ws + l.o[mode]);
+    a.part_m = reinterpret_cast<float*>(ws + l.m[mode]);
+    a.part_l = reinterpret_cast<float*>(ws + l.l[mode]);
+  };
+  place(0);
+  AttnArgs split = a;
+  place(1);
   a.arrived = ctx->d_attn_cnt;
   const bool bf16 = desc->dtype == MDLC_BF16;
   cudaError_t e;
-  if (padded_dim(desc->head_dim) == 64) e = bf16 ? run_attn<__nv_bfloat16, 64>(ctx, a) : run_attn<float, 64>(ctx, a);
-  else e = bf16 ? run_attn<__nv_bfloat16, 128>(ctx, a) : run_attn<float, 128>(ctx, a);
+  split.arrived = a.arrived;
+  if (padded_dim(desc->head_dim) == 64) e = bf16 ? run_attn<__nv_bfloat16, 64>(ctx, split, a) : run_attn<float, 64>(ctx, split, a);
+  else e = bf16 ? run_attn<__nv_bfloat16, 128>(ctx, split, a) : run_attn<float, 128>(ctx, split, a);
   return mdlc_cuda_status(ctx, e, "paged_attn launch");
 }

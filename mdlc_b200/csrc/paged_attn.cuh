@@ -7,6 +7,13 @@
 
 namespace mdlc {
 
+// n / d for 0 <= n < 65536 and 1 <= d <= 65536 as a product: a runtime division costs some 20 instructions
+struct SmallDiv {
+  uint32_t m;  // ceil(2^32 / d), 0 for d = 1
+};
+inline SmallDiv small_div(int d) { return {d == 1 ? 0u : 0xffffffffu / (uint32_t)d + 1u}; }
+MDLC_DEV int div_small(int n, const SmallDiv& s) { return s.m ? (int)__umulhi((uint32_t)n, s.m) : n; }
+
 struct AttnArgs {
   mdlc_attn_desc d;
   const void *q, *k, *v;
@@ -14,8 +21,10 @@ struct AttnArgs {
   void* out;
   float* lse;
   int group;          // query heads per key head
+  SmallDiv group_div;
   int split_rows;     // requests with at most this many rows go to split mode
   int splits;         // chunk mode: blocks that may share a row tile's keys
+  int beside;         // chunk mode: runs beside the split kernel in front of it, see chunk_begin
   float scale_log2;   // scale * log2(e)
   // workspace: partial sums [slot][rows][hdp], their maxima (base-2 exponent) and sums [slot][rows]
   float *part_o, *part_m, *part_l;
@@ -126,6 +135,18 @@ MDLC_DEV bool find_tile(const AttnArgs& a, long long want, int tile_rows, long l
   t->rows = t->rq.q_len * a.group;
   return true;
 }
+// Chunk mode after split mode in one call: the two touch different rows and parts of the workspace, so a chunk block need
+// not wait for the split kernel to end. It starts once every split block has let dependents go, which they do
+// after their own wait, so all work before the call is done and visible. The kernel after this one waits for this one alone:
+// one block therefore waits for the split kernel before it ends.
+MDLC_DEV void chunk_begin(const AttnArgs& a) {
+  if (!a.beside) pdl_wait();
+  pdl_trigger();
+}
+MDLC_DEV void chunk_end(const AttnArgs& a) {
+  if (a.beside && (blockIdx.x | blockIdx.y | blockIdx.z) == 0) pdl_wait();
+}
+
 // blocks that share a tile of n key blocks: each gets at least two
 MDLC_DEV int splits_of(const AttnArgs& a, int n, int least) { return max(1, min(a.splits, n / least)); }
 

@@ -141,22 +141,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
   const mdlc_attn_desc& d = a.d;
   volatile int* abort_flag = &abort_s;
 
+  // what touches no global memory comes before the wait for the kernel in front
   if (warp == 9 && lane == 0) {
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
   }
-  pdl_wait();
-  pdl_trigger();
-  Tile t;
-  if (!find_tile(a, blockIdx.y, kRows, warp_sums, &place_s, &t)) return;
-  const int e = blockIdx.x;
-  const Span sp = span_of(a, t.rq, t.r0 / a.group, (min(t.r0 + kRows, t.rows) - 1) / a.group, kKeys);
-  const int ns = splits_of(a, sp.n, 2);
-  if ((int)blockIdx.z >= ns) return;
-  const int blk0 = (int)((long long)blockIdx.z * sp.n / ns), blk1 = (int)((long long)(blockIdx.z + 1) * sp.n / ns), nb = blk1 - blk0;
-  const int shift = t.rq.kv_len - t.rq.q_len;
-  const int n_tiles = t.rows - t.r0 > 128 ? 2 : 1;
-
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(bar(kFull + i), 1);
@@ -173,6 +162,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
     abort_s = missing_s = 0;
     fence_mbar_init();
   }
+  chunk_begin(a);
+  Tile t;
+  if (!find_tile(a, blockIdx.y, kRows, warp_sums, &place_s, &t)) return chunk_end(a);
+  const int e = blockIdx.x;
+  const Span sp = span_of(a, t.rq, t.r0 / a.group, (min(t.r0 + kRows, t.rows) - 1) / a.group, kKeys);
+  const int ns = splits_of(a, sp.n, 2);
+  if ((int)blockIdx.z >= ns) return;  // (the first share always has work)
+  const int blk0 = (int)((long long)blockIdx.z * sp.n / ns), blk1 = (int)((long long)(blockIdx.z + 1) * sp.n / ns), nb = blk1 - blk0;
+  const int shift = t.rq.kv_len - t.rq.q_len;
+  const int n_tiles = t.rows - t.r0 > 128 ? 2 : 1;
   if (warp == 8) {
     tmem_alloc(smem_u32(&tmem_s), 512);
     tmem_relinquish();
@@ -181,6 +180,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_s;  // all 512 columns: 0, which the MMA warp takes for granted
+  // token and head of row t.r0 + rl (rl < 256): the tile's first ones, and a division of a small number
+  const int tok0 = t.r0 / a.group, rem0 = t.r0 - tok0 * a.group;
+  auto token_of = [&](int rl, int* head) {
+    const int n = div_small(rem0 + rl, a.group_div);
+    *head = e * a.group + rem0 + rl - n * a.group;
+    return t.rq.q0 + tok0 + n;
+  };
 
   if (warp < 8) {
     // ------------------------------------------------------------ softmax
@@ -193,11 +199,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
         uint4 v[8];
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
-          const int i = i0 + n * 256, rl = i / CH, c = i % CH, r = t.r0 + rl;
+          const int i = i0 + n * 256, rl = i / CH, c = i % CH;
           v[n] = make_uint4(0, 0, 0, 0);
-          if (r < t.rows && c < chunks)
-            v[n] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + (long long)(t.rq.q0 + r / a.group) * d.q_stride +
-                                                        (long long)(e * a.group + r % a.group) * d.head_dim) + c);
+          if (t.r0 + rl < t.rows && c < chunks) {
+            int head;
+            const int tok = token_of(rl, &head);
+            v[n] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + tok * d.q_stride + (long long)head * d.head_dim) + c);
+          }
         }
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
@@ -208,11 +216,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
       fence_proxy_async_smem();
       mbar_arrive(bar(kQ));
     }
+    const int page_log2 = 31 - __clz(d.page);  // a power of two
     // Ids that do not exist hide their keys: looked for once, so that the blocks need not look (a load from the table
     // in front of every block cost 570 cycles of 4200)
     auto missing = [&](int j) {
       return j < sp.hi && (j + min(d.page, kKeys) > sp.lo || j < d.sinks) &&
-             (unsigned)__ldg(a.table + (long long)t.b * d.table_stride + j / d.page) >= (unsigned)d.pages;
+             (unsigned)__ldg(a.table + (long long)t.b * d.table_stride + (j >> page_log2)) >= (unsigned)d.pages;
     };
     {
       const int per = kKeys / min(d.page, kKeys);
@@ -334,10 +343,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
       tc_fence_after();
       if (ok) {
         const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-        const int tok = t.rq.q0 + r / a.group, head = e * a.group + r % a.group;
         const long long slot = (((long long)blockIdx.y * d.kv_heads + e) * a.splits + blockIdx.z) * kRows + rl;
         const float mlog = m == -INFINITY ? -INFINITY : m * c;
-        __nv_bfloat16* po = static_cast<__nv_bfloat16*>(a.out) + (long long)tok * d.out_stride + (long long)head * d.head_dim;
         uint32_t o[HDP];
 #pragma unroll
         for (int i = 0; i < HDP; ++i) o[i] = 0;
@@ -346,16 +353,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
           for (int i = 0; i < HDP; i += 32) tmem_ld32(o_addr + i, o + i);
           tmem_ld_wait();
         }
-        if (live && ns == 1) {
+        if (ns == 1) {
+          // through the place of this warp's queries (their products are done), so that rows are written whole
+          constexpr int CH = HDP / 8;
+          unsigned char* rows = smem + C::Q + tile * C::TILE + (warp & 3) * 32 * HDP * 2;
 #pragma unroll
-          for (int k = 0; k < HDP; k += 8) {
-            if (k < d.head_dim) {
-              uint4 v;
-              v.x = pack_bf16x2(__uint_as_float(o[k]) * inv, __uint_as_float(o[k + 1]) * inv);
-              v.y = pack_bf16x2(__uint_as_float(o[k + 2]) * inv, __uint_as_float(o[k + 3]) * inv);
-              v.z = pack_bf16x2(__uint_as_float(o[k + 4]) * inv, __uint_as_float(o[k + 5]) * inv);
-              v.w = pack_bf16x2(__uint_as_float(o[k + 6]) * inv, __uint_as_float(o[k + 7]) * inv);
-              *reinterpret_cast<uint4*>(po + k) = v;
+          for (int k = 0; k < CH; ++k) {
+            uint4 v;
+            v.x = pack_bf16x2(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv);
+            v.y = pack_bf16x2(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
+            v.z = pack_bf16x2(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
+            v.w = pack_bf16x2(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
+            *reinterpret_cast<uint4*>(rows + lane * HDP * 2 + ((k ^ (lane & 7)) << 4)) = v;
+          }
+          __syncwarp();
+#pragma unroll 4
+          for (int i = lane; i < 32 * CH; i += 32) {
+            const int row = i / CH, k = i % CH, rw = warp * 32 + row;
+            if (t.r0 + rw < t.rows && 8 * k < d.head_dim) {
+              int head;
+              const int tok = token_of(rw, &head);
+              *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + tok * d.out_stride + (long long)head * d.head_dim + 8 * k) =
+                  *reinterpret_cast<const uint4*>(rows + row * HDP * 2 + ((k ^ (row & 7)) << 4));
             }
           }
         } else if (live) {
@@ -368,7 +387,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
             a.part_m[slot] = mlog;
             a.part_l[slot] = l;
           } else if (a.lse) {
-            a.lse[(long long)tok * d.heads + head] = (mlog + log2f(l)) * 0.69314718055994531f;
+            int head;
+            const long long tok = token_of(rl, &head);
+            a.lse[tok * d.heads + head] = (mlog + log2f(l)) * 0.69314718055994531f;
           }
         }
       }
@@ -478,6 +499,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
       // given up: this block's copies must land before its shared memory goes back
       for (int i = max(0, u - kRing); i < u; ++i) mbar_wait(bar(kFull + i % kRing), (i / kRing) & 1, nullptr, err, kWaitCycles);
     }
+    } else if (warp == 10) {
+      chunk_end(a);  // the block ends after this warp
     }
   }
   __syncwarp();
@@ -517,7 +540,7 @@ cudaError_t attn_tensor_maps(const AttnArgs& a, int box, CUtensorMap* k, CUtenso
 // bf16, pages that tile a 128-key block, a positive scale (the running maximum is that of the raw scores)
 bool attn_tc_fits(const mdlc_attn_desc& d) {
   const bool page = d.page >= 8 && (d.page & (d.page - 1)) == 0;
-  return d.dtype == MDLC_BF16 && page && d.scale > 0.0f;
+  return d.dtype == MDLC_BF16 && page && d.scale > 0.0f && d.heads / d.kv_heads <= 4096;  // (small divisions by the group)
 }
 
 cudaError_t attn_tc_launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid) {
