@@ -461,7 +461,8 @@ int mdlc_rope_append(mdlc_ctx* ctx, const mdlc_rope_desc* desc, const void* q, c
  * optional, [tokens][heads] fp32, may be null). Table entries of pages that no new
  * token sees (behind the window, past kv_lens) are not read. A page id
  * outside [0, pages) among the read ones counts as hidden keys. Keys and values
- * past kv_lens may hold anything, NaN included. Rows past q_starts[batch] are left
+ * past kv_lens may hold anything, NaN included; a non-finite one within it may reach
+ * tokens that do not see it (as 0 x inf). Rows past q_starts[batch] are left
  * as they are. `workspace`: mdlc_paged_attn_workspace bytes, 16-byte aligned, for
  * this call alone. q, out and caches are 16-byte aligned, the strides multiples of 8
  * elements. max_q and max_kv bound every request's q_len and kv_len: longer ones
@@ -487,10 +488,12 @@ int mdlc_paged_attn(mdlc_ctx* ctx, const mdlc_attn_desc* desc, const void* q, co
  *   y[i][o] = bias[o] + sum_c x[i][c] (code[o][c] - zero[o][c / group]) scale[o][c / group]
  * codes: [n][k / 2] bytes, column c in the low (c even) or high (c odd) nibble of
  * byte c / 2; scales: [n][k / group] bf16; zeros: [n][k / group] uint8 0..15, null:
- * 8; bias: [n] fp32 or null. Products are exact, sums in fp32 (an fp32 x is taken
- * as three bf16 parts). codes 16-byte aligned; x 16-byte aligned with x_stride a multiple of 8. */
+ * 8; bias: [n] fp32 or null. x is taken to 23 bits of the largest |x| of each row's 128
+ * columns (what an fp32 product with that one would round), products and a group's sums
+ * are exact, groups are added in fp32; a non-finite x gives a non-finite y. codes 16-byte
+ * aligned; x 16-byte aligned with x_stride a multiple of 8. Uses the context's split-K workspace. */
 typedef struct {
-  int32_t m;     /* rows; made for 1 .. 32, more re-read the weights */
+  int32_t m;     /* rows, at most 65535; made for 1 .. 16, more re-read the weights */
   int32_t n;     /* output columns */
   int32_t k;     /* a multiple of group */
   int32_t group; /* 32, 64 or 128 */
