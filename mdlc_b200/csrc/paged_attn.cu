@@ -888,11 +888,11 @@ Chunk chunk_of(const mdlc_attn_desc& d) {
   const int group = d.heads / d.kv_heads;
   Chunk c = {};
   c.used = (long long)d.max_q * group > 16 * split_groups(d);
-  c.tc = attn_tc_fits(d) && (long long)d.tokens * group / kTcRows + d.batch <= 65535;  // the tiles are its grid's y
-  c.rows = c.tc ? kTcRows : 64;
+  c.tc = attn_tc_fits(d) && (long long)d.tokens * group / attn_tc_rows(d.head_dim) + d.batch <= 65535;  // the tiles are its grid's y
+  c.rows = c.tc ? attn_tc_rows(d.head_dim) : 64;
   c.tiles = (int)min((long long)d.tokens * group / c.rows + d.batch, (long long)INT32_MAX);
-  // the mma.sync kernel runs three blocks per SM
-  const long long room = kChunkBlocks * (c.tc ? 1 : 3) / ((long long)c.tiles * d.kv_heads);
+  // blocks on an SM: two of one row tile, one of two; three of the mma.sync kernel's
+  const long long room = kChunkBlocks * (c.tc ? (c.rows == 128 ? 2 : 1) : 3) / ((long long)c.tiles * d.kv_heads);
   c.splits = (int)max(1ll, min(room, min(16ll, (long long)d.max_kv / kLeastKeys)));
   return c;
 }
@@ -945,7 +945,7 @@ cudaError_t run_split(mdlc_ctx* ctx, const AttnArgs& a) {
 }
 
 template <int HDP, int NT>
-cudaError_t run_narrow(mdlc_ctx* ctx, const AttnArgs& a) {
+cudaError_t run_narrow(mdlc_ctx* ctx, const AttnArgs& a, bool chunks) {
   using C = NarrowCfg<HDP, NT>;
   CUtensorMap maps[2];
   cudaError_t e = attn_tensor_maps(a, min(a.d.page, C::BT), &maps[0], &maps[1]);
@@ -953,7 +953,8 @@ cudaError_t run_narrow(mdlc_ctx* ctx, const AttnArgs& a) {
   static SmemLimit seen;
   e = allow_smem(seen, ctx->device, attn_narrow_kernel<HDP, NT>, C::SMEM);
   if (e != cudaSuccess) return e;
-  const int blocks = min(kMaxBlocks, ctx->num_sms * (C::SMEM <= 100 * 1024 ? 2 : 1));
+  // two blocks per SM; one where chunks of the same call run beside
+  const int blocks = min(kMaxBlocks, ctx->num_sms * (C::SMEM <= 100 * 1024 && !chunks ? 2 : 1));
   mdlc_note_launch(ctx);
   return launch_pdl(attn_narrow_kernel<HDP, NT>, dim3(blocks), dim3(kAttnThreads), C::SMEM, ctx->stream, a, maps[0], maps[1], ctx->d_err);
 }
@@ -964,12 +965,13 @@ bool narrow_fits(const mdlc_attn_desc& d) { return d.dtype == MDLC_BF16 && d.pag
 template <typename T, int HDP>
 cudaError_t run_attn(mdlc_ctx* ctx, AttnArgs& sa, AttnArgs& a) {  // split mode's and chunk mode's arguments
   const int wm = split_groups(a.d);
+  const Chunk c = chunk_of(a.d);
   cudaError_t e = cudaSuccess;
   if (wm == 1 && narrow_fits(a.d)) {
     // requests of up to 8 rows in one column tile; with more than 8 heads per key head, or several tokens, two
     const bool one = a.group <= 8 && ((long long)a.d.max_q * a.group <= 8 || (long long)a.d.max_q * a.group > 16);
     if (one) sa.split_rows = a.split_rows = 8;
-    e = one ? run_narrow<HDP, 1>(ctx, sa) : run_narrow<HDP, 2>(ctx, sa);
+    e = one ? run_narrow<HDP, 1>(ctx, sa, c.used) : run_narrow<HDP, 2>(ctx, sa, c.used);
   } else if (wm == 1) {
     e = run_split<T, HDP, 1>(ctx, sa);
   } else if (wm == 2) {
@@ -977,7 +979,6 @@ cudaError_t run_attn(mdlc_ctx* ctx, AttnArgs& sa, AttnArgs& a) {  // split mode'
   } else if (wm == 4) {
     e = run_split<T, HDP, 4>(ctx, sa);
   }
-  const Chunk c = chunk_of(a.d);
   if (e != cudaSuccess || !c.used) return e;
   a.splits = c.splits;
   a.beside = wm > 0;

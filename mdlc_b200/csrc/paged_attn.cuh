@@ -31,8 +31,9 @@ struct AttnArgs {
   int* arrived;           // split mode: arrivals at the tile that starts in block c and others share
 };
 
-// chunk mode on the tensor cores' tcgen05 form (bf16): rows of a tile, keys of a block
-constexpr int kTcRows = 256, kTcKeys = 128;
+// chunk mode on the tensor cores' tcgen05 form (bf16): keys of a block, rows of a block
+constexpr int kTcKeys = 128;
+int attn_tc_rows(int head_dim);
 bool attn_tc_fits(const mdlc_attn_desc& d);
 cudaError_t attn_tc_launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid);
 // tensor maps of the two caches (rows of head_dim elements) with boxes of `box` rows x 64 columns, 128-byte swizzle

@@ -2,8 +2,8 @@
 //
 // A block takes 256 rows (two tiles of 128, one per softmax warpgroup) of one key head, so that
 // the 64 KB of keys and values of a 128-key block that it reads from L2 serve
-// 256 rows: 4 x 256 x 128 x d operations per 512 d bytes. Roles:
-//   warps 0-3, 4-7  softmax of row tile 0 / 1: a thread owns a row, reads its 128 scores from
+// 256 rows: 4 x 256 x 128 x d operations per 512 d bytes. (Heads of up to 64 columns: one tile, two blocks per SM.) Roles, for two tiles:
+//   warps 0-3, 4-7  softmax of row tile 0 / 1: a thread owns a row, reads its scores from
 //                   tensor memory, keeps the running maximum and sum, writes the weights back
 //                   to tensor memory as bf16 (the A operand of the second product)
 //   warp 8          issues every MMA (one thread) and owns the tensor memory
@@ -26,23 +26,28 @@
 namespace mdlc {
 namespace {
 
-constexpr int kThreads = 384;
-// registers of a softmax and of another thread: 2 x 128 x 208 + 128 x 88 = 384 x 168, what the block is launched with
-constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
-constexpr int kRows = kTcRows, kKeys = kTcKeys;
+constexpr int kKeys = kTcKeys;
 constexpr int kRing = 4;             // key / value tiles in shared memory: K(j), V(j), K(j+1), V(j+1)
 constexpr float kGrow = 8.0f;        // growth of a row's maximum (base-2 exponent) that rescales the output
 constexpr unsigned long long kWaitCycles = 2 * kWaitLimitNs;
 
 template <int HDP>
 struct TcCfg {
+  // Row tiles of a block. Heads of up to 64 columns: one, since two such blocks fit on an SM and one's prologue and end overlap the
+  // other's work; wider ones: two, for which a key block is read from L2 once.
+  static constexpr int TILES = HDP == 64 ? 1 : 2;
+  static constexpr int ROWS = 128 * TILES, SOFT = 4 * TILES;  // rows; softmax warps, in front of the four others
+  static constexpr int THREADS = 128 * TILES + 128;
+  // registers of a softmax and of another thread; their sum is what the block is launched with: 128 x (168 + 88) = 256 x 128,
+  // 2 x 128 x 208 + 128 x 88 = 384 x 168
+  static constexpr int SOFT_REGS = TILES == 1 ? 168 : 208, OTHER_REGS = 88;
   static constexpr int HALVES = HDP / 64;               // 128-byte wide column blocks
   static constexpr int TILE = 128 * HDP * 2;            // one Q tile, one key or value tile
   static constexpr int Q = 0;
-  static constexpr int RING = 2 * TILE;
+  static constexpr int RING = TILES * TILE;
   static constexpr int BARS = RING + kRing * TILE;
   static constexpr int SMEM = BARS + 256 + 1024;        // 1024: alignment of the base
-  static constexpr int O_COL = 256;
+  static constexpr int O_COL = 128 * TILES, TMEM = 256 * TILES;  // outputs' first column; columns in all
 };
 // barriers; scores, weights and outputs have one per row tile and half of the key block (kS + 2 tile + half, ...)
 enum { kFull = 0, kEmpty = kRing, kRaw = 2 * kRing, kQ, kS, kP = kS + 4, kO = kP + 4, kDrain = kO + 4, kBars };
@@ -126,11 +131,11 @@ MDLC_DEV float ex2(float x) {
 }
 
 template <int HDP>
-__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
+__global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) attn_tc_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap,
                                                               const __grid_constant__ CUtensorMap vmap, int* err) {
   using C = TcCfg<HDP>;
   extern __shared__ unsigned char tc_smem_raw[];
-  __shared__ long long warp_sums[kThreads / 32];
+  __shared__ long long warp_sums[C::THREADS / 32];
   __shared__ Place place_s;
   __shared__ uint32_t tmem_s;
   __shared__ int abort_s, missing_s;
@@ -142,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
   volatile int* abort_flag = &abort_s;
 
   // what touches no global memory comes before the wait for the kernel in front
-  if (warp == 9 && lane == 0) {
+  if (warp == C::SOFT + 1 && lane == 0) {
     tma_prefetch_desc(&kmap);
     tma_prefetch_desc(&vmap);
   }
@@ -152,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
       mbar_init(bar(kEmpty + i), 1);
     }
     mbar_init(bar(kRaw), 1);
-    mbar_init(bar(kQ), 256);
+    mbar_init(bar(kQ), C::ROWS);
     for (int i = 0; i < 4; ++i) {
       mbar_init(bar(kS + i), 1);
       mbar_init(bar(kP + i), 128);
@@ -164,23 +169,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
   }
   chunk_begin(a);
   Tile t;
-  if (!find_tile(a, blockIdx.y, kRows, warp_sums, &place_s, &t)) return chunk_end(a);
+  if (!find_tile(a, blockIdx.y, C::ROWS, warp_sums, &place_s, &t)) return chunk_end(a);
   const int e = blockIdx.x;
-  const Span sp = span_of(a, t.rq, t.r0 / a.group, (min(t.r0 + kRows, t.rows) - 1) / a.group, kKeys);
+  const Span sp = span_of(a, t.rq, t.r0 / a.group, (min(t.r0 + C::ROWS, t.rows) - 1) / a.group, kKeys);
   const int ns = splits_of(a, sp.n, 2);
   if ((int)blockIdx.z >= ns) return;  // (the first share always has work)
   const int blk0 = (int)((long long)blockIdx.z * sp.n / ns), blk1 = (int)((long long)(blockIdx.z + 1) * sp.n / ns), nb = blk1 - blk0;
   const int shift = t.rq.kv_len - t.rq.q_len;
-  const int n_tiles = t.rows - t.r0 > 128 ? 2 : 1;
-  if (warp == 8) {
-    tmem_alloc(smem_u32(&tmem_s), 512);
+  const int n_tiles = C::TILES == 2 && t.rows - t.r0 > 128 ? 2 : 1;
+  if (warp == C::SOFT) {
+    tmem_alloc(smem_u32(&tmem_s), C::TMEM);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = tmem_s;  // all 512 columns: 0, which the MMA warp takes for granted
-  // token and head of row t.r0 + rl (rl < 256): the tile's first ones, and a division of a small number
+  const uint32_t tmem = tmem_s;
+  // token and head of row t.r0 + rl: the tile's first ones, and a division of a small number
   const int tok0 = t.r0 / a.group, rem0 = t.r0 - tok0 * a.group;
   auto token_of = [&](int rl, int* head) {
     const int n = div_small(rem0 + rl, a.group_div);
@@ -188,18 +193,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
     return t.rq.q0 + tok0 + n;
   };
 
-  if (warp < 8) {
+  if (warp < C::SOFT) {
     // ------------------------------------------------------------ softmax
-    regs_up<kSoftmaxRegs>();
+    regs_up<C::SOFT_REGS>();
     // queries: rows of 128 bytes per 64 columns, 16-byte chunks swizzled by the row
     {
       const int chunks = d.head_dim / 8;
       constexpr int CH = HDP / 8;
-      for (int i0 = threadIdx.x; i0 < kRows * CH; i0 += 8 * 256) {  // eight loads at a time
+      for (int i0 = threadIdx.x; i0 < C::ROWS * CH; i0 += 8 * C::ROWS) {  // eight loads at a time
         uint4 v[8];
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
-          const int i = i0 + n * 256, rl = i / CH, c = i % CH;
+          const int i = i0 + n * C::ROWS, rl = i / CH, c = i % CH;
           v[n] = make_uint4(0, 0, 0, 0);
           if (t.r0 + rl < t.rows && c < chunks) {
             int head;
@@ -209,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
         }
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
-          const int i = i0 + n * 256, rl = i / CH, c = i % CH;
+          const int i = i0 + n * C::ROWS, rl = i / CH, c = i % CH;
           *reinterpret_cast<uint4*>(smem + C::Q + (rl >> 7) * C::TILE + (c >> 3) * 16384 + (rl & 127) * 128 + (((c & 7) ^ (rl & 7)) << 4)) = v[n];
         }
       }
@@ -226,9 +231,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
     {
       const int per = kKeys / min(d.page, kKeys);
       bool none = false;
-      for (int i = threadIdx.x; i < nb * per; i += 256) none |= missing(key_of_block(sp, blk0 + i / per, kKeys) + i % per * min(d.page, kKeys));
+      for (int i = threadIdx.x; i < nb * per; i += C::ROWS) none |= missing(key_of_block(sp, blk0 + i / per, kKeys) + i % per * min(d.page, kKeys));
       if (none) missing_s = 1;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
+      asm volatile("bar.sync 1, %0;" ::"n"(C::ROWS) : "memory");
     }
     const bool any_missing = *(volatile int*)&missing_s;
     const int tile = warp >> 2, rl = threadIdx.x, r = t.r0 + rl;
@@ -343,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
       tc_fence_after();
       if (ok) {
         const float inv = l > 0.0f ? 1.0f / l : (l == 0.0f ? 0.0f : l);
-        const long long slot = (((long long)blockIdx.y * d.kv_heads + e) * a.splits + blockIdx.z) * kRows + rl;
+        const long long slot = (((long long)blockIdx.y * d.kv_heads + e) * a.splits + blockIdx.z) * C::ROWS + rl;
         const float mlog = m == -INFINITY ? -INFINITY : m * c;
         uint32_t o[HDP];
 #pragma unroll
@@ -395,11 +400,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
       }
     }
   } else {
-    regs_down<kOtherRegs>();  // warps 8 to 11 alike, before their ways part
-    if (warp == 8) {
+    regs_down<C::OTHER_REGS>();  // the last four warps alike, before their ways part
+    if (warp == C::SOFT) {
     // ------------------------------------------------------------ MMA
     const uint32_t leader = elect_leader();
     const int u_nb = __shfl_sync(0xffffffffu, nb, 0), u_tiles = __shfl_sync(0xffffffffu, n_tiles, 0);
+    const uint32_t u_tmem = __shfl_sync(0xffffffffu, tmem, 0);
     if (u_nb > 0) {
       constexpr uint32_t kIdS = idesc_bf16(128, 64), kIdO = idesc_bf16_nmajor(128, HDP);
       bool ok = __all_sync(0xffffffffu, mbar_wait(bar(kQ), 0, abort_flag, err, kWaitCycles));
@@ -409,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
 #pragma unroll
         for (int ks = 0; ks < HDP / 16; ++ks) {
           const uint32_t off = (ks / 4) * 16384 + (ks % 4) * 32;
-          umma_lead(leader, i * 128 + h * 64, umma_desc_sw128(q + off), umma_desc_sw128(k + off), kIdS, ks > 0);
+          umma_lead(leader, u_tmem + i * 128 + h * 64, umma_desc_sw128(q + off), umma_desc_sw128(k + off), kIdS, ks > 0);
         }
         commit_lead(leader, bar(kS + 2 * i + h));
       };
@@ -430,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
             tc_fence_after();
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
-              umma_lead_ta(leader, C::O_COL + i * HDP, i * 128 + h * 64 + ks * 8, umma_desc_sw128_n(v + (4 * h + ks) * 2048, 16384), kIdO,
+              umma_lead_ta(leader, u_tmem + C::O_COL + i * HDP, u_tmem + i * 128 + h * 64 + ks * 8, umma_desc_sw128_n(v + (4 * h + ks) * 2048, 16384), kIdO,
                            j > 0 || h > 0 || ks > 0);
             commit_lead(leader, bar(kO + 2 * i + h));
             const bool last = h == 1 && i == u_tiles - 1;
@@ -451,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
       mbar_wait(bar(kDrain), 0, nullptr, err, kWaitCycles);
     }
     __syncwarp();
-    } else if (warp == 9) {
+    } else if (warp == C::SOFT + 1) {
     // ------------------------------------------------------------ keys and values
     const int box = min(d.page, kKeys), boxes = kKeys / box;
     const int page_i = lane % boxes, half = lane / boxes;   // this lane's box: boxes x HALVES <= 32 of them
@@ -499,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
       // given up: this block's copies must land before its shared memory goes back
       for (int i = max(0, u - kRing); i < u; ++i) mbar_wait(bar(kFull + i % kRing), (i / kRing) & 1, nullptr, err, kWaitCycles);
     }
-    } else if (warp == 10) {
+    } else if (warp == C::SOFT + 2) {
       chunk_end(a);  // the block ends after this warp
     }
   }
@@ -507,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 8) tmem_dealloc(tmem, 512);
+  if (warp == C::SOFT) tmem_dealloc(tmem, C::TMEM);
 }
 
 template <int HDP>
@@ -519,7 +525,7 @@ cudaError_t launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid) {
   e = allow_smem(seen, ctx->device, attn_tc_kernel<HDP>, TcCfg<HDP>::SMEM);
   if (e != cudaSuccess) return e;
   // key heads fastest: the tiles that see the most keys start first in all of them
-  return launch_pdl(attn_tc_kernel<HDP>, dim3(grid.y, grid.x, grid.z), dim3(kThreads), TcCfg<HDP>::SMEM, ctx->stream, a, maps[0], maps[1], ctx->d_err);
+  return launch_pdl(attn_tc_kernel<HDP>, dim3(grid.y, grid.x, grid.z), dim3(TcCfg<HDP>::THREADS), TcCfg<HDP>::SMEM, ctx->stream, a, maps[0], maps[1], ctx->d_err);
 }
 
 }  // namespace
@@ -542,6 +548,8 @@ bool attn_tc_fits(const mdlc_attn_desc& d) {
   const bool page = d.page >= 8 && (d.page & (d.page - 1)) == 0;
   return d.dtype == MDLC_BF16 && page && d.scale > 0.0f && d.heads / d.kv_heads <= 4096;  // (small divisions by the group)
 }
+
+int attn_tc_rows(int head_dim) { return head_dim <= 64 ? TcCfg<64>::ROWS : TcCfg<128>::ROWS; }
 
 cudaError_t attn_tc_launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid) {
   return a.d.head_dim <= 64 ? launch<64>(ctx, a, grid) : launch<128>(ctx, a, grid);
