@@ -6,9 +6,9 @@
 //   warps 0-3, 4-7  softmax of row tile 0 / 1: a thread owns a row, reads its scores from
 //                   tensor memory, keeps the running maximum and sum, writes the weights back
 //                   to tensor memory as bf16 (the A operand of the second product)
-//   warp 8          issues every MMA (one thread) and owns the tensor memory
+//   warps 8, 10     issue the MMAs (one thread each) of row tile 0 / 1; warp 8 owns the tensor memory
 //   warp 9          loads keys and values by TMA, a box per page, 32 lanes at once
-//   (warps 8-11 give registers to the softmax warpgroups; 10 and 11 do nothing else)
+//   (warps 8-11 give registers to the softmax warpgroups)
 // Tensor memory (512 columns): scores of the two tiles [0, 256), 64 columns per half of a key block, the weights over the
 // first 32 of their own half's; outputs [256, 256 + 2 HDP). Per half n of a key block the MMAs are O += P(n) V(n), then the scores of
 // half n + 2 into the place that P(n) leaves (issue order makes them overwrite it only after it was read): a tile always has the next half's
@@ -50,7 +50,7 @@ struct TcCfg {
   static constexpr int O_COL = 128 * TILES, TMEM = 256 * TILES;  // outputs' first column; columns in all
 };
 // barriers; scores, weights and outputs have one per row tile and half of the key block (kS + 2 tile + half, ...)
-enum { kFull = 0, kEmpty = kRing, kRaw = 2 * kRing, kQ, kS, kP = kS + 4, kO = kP + 4, kDrain = kO + 4, kBars };
+enum { kFull = 0, kEmpty = kRing, kRaw = 2 * kRing, kQ, kS, kP = kS + 4, kO = kP + 4, kDrain = kO + 4, kBars = kDrain + 2 };
 
 // instruction descriptor: bf16 x bf16 -> fp32; B stored along its N axis (values)
 constexpr uint32_t idesc_bf16_nmajor(int M, int N) { return idesc_bf16(M, N) | (1u << 16); }
@@ -154,7 +154,6 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(bar(kFull + i), 1);
-      mbar_init(bar(kEmpty + i), 1);
     }
     mbar_init(bar(kRaw), 1);
     mbar_init(bar(kQ), C::ROWS);
@@ -163,7 +162,7 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
       mbar_init(bar(kP + i), 128);
       mbar_init(bar(kO + i), 1);
     }
-    mbar_init(bar(kDrain), 1);
+    for (int i = 0; i < C::TILES; ++i) mbar_init(bar(kDrain + i), 1);
     abort_s = missing_s = 0;
     fence_mbar_init();
   }
@@ -177,6 +176,10 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
   const int blk0 = (int)((long long)blockIdx.z * sp.n / ns), blk1 = (int)((long long)(blockIdx.z + 1) * sp.n / ns), nb = blk1 - blk0;
   const int shift = t.rq.kv_len - t.rq.q_len;
   const int n_tiles = C::TILES == 2 && t.rows - t.r0 > 128 ? 2 : 1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kRing; ++i) mbar_init(bar(kEmpty + i), n_tiles);  // both tiles' MMAs give a key or value tile back
+    fence_mbar_init();
+  }
   if (warp == C::SOFT) {
     tmem_alloc(smem_u32(&tmem_s), C::TMEM);
     tmem_relinquish();
@@ -401,60 +404,58 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
     }
   } else {
     regs_down<C::OTHER_REGS>();  // the last four warps alike, before their ways part
-    if (warp == C::SOFT) {
-    // ------------------------------------------------------------ MMA
+    if (warp == C::SOFT || (C::TILES == 2 && warp == C::SOFT + 2)) {
+    // ------------------------------------------------------------ MMA: a warp per row tile
     const uint32_t leader = elect_leader();
-    const int u_nb = __shfl_sync(0xffffffffu, nb, 0), u_tiles = __shfl_sync(0xffffffffu, n_tiles, 0);
-    const uint32_t u_tmem = __shfl_sync(0xffffffffu, tmem, 0);
+    const int i = warp == C::SOFT ? 0 : 1;
+    const int u_nb = __shfl_sync(0xffffffffu, i < n_tiles ? nb : 0, 0);
+    const uint32_t u_s = __shfl_sync(0xffffffffu, tmem + i * 128, 0), u_o = __shfl_sync(0xffffffffu, tmem + C::O_COL + i * HDP, 0);
     if (u_nb > 0) {
       constexpr uint32_t kIdS = idesc_bf16(128, 64), kIdO = idesc_bf16_nmajor(128, HDP);
       bool ok = __all_sync(0xffffffffu, mbar_wait(bar(kQ), 0, abort_flag, err, kWaitCycles));
       auto wait_tile = [&](int u) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar(kFull + u % kRing), (u / kRing) & 1, abort_flag, err, kWaitCycles)); };
-      auto scores = [&](int i, int j, int h) {  // half h of S_i = Q_i K(j)^T
+      auto scores = [&](int j, int h) {  // half h of S = Q K(j)^T
         const uint32_t q = sbase + C::Q + i * C::TILE, k = sbase + C::RING + ((2 * j) % kRing) * C::TILE + h * 8192;
 #pragma unroll
         for (int ks = 0; ks < HDP / 16; ++ks) {
           const uint32_t off = (ks / 4) * 16384 + (ks % 4) * 32;
-          umma_lead(leader, u_tmem + i * 128 + h * 64, umma_desc_sw128(q + off), umma_desc_sw128(k + off), kIdS, ks > 0);
+          umma_lead(leader, u_s + h * 64, umma_desc_sw128(q + off), umma_desc_sw128(k + off), kIdS, ks > 0);
         }
         commit_lead(leader, bar(kS + 2 * i + h));
       };
       ok = ok && wait_tile(0);
       tc_fence_after();
       if (ok) {
-        for (int h = 0; h < 2; ++h)
-          for (int i = 0; i < u_tiles; ++i) scores(i, 0, h);
+        scores(0, 0);
+        scores(0, 1);
         commit_lead(leader, bar(kEmpty + 0));
       }
       for (int j = 0; ok && j < u_nb; ++j) {
         ok = wait_tile(2 * j + 1);
         const uint32_t v = sbase + C::RING + ((2 * j + 1) % kRing) * C::TILE;
-        for (int h = 0; ok && h < 2; ++h)
-          for (int i = 0; i < u_tiles; ++i) {
-            ok = __all_sync(0xffffffffu, mbar_wait(bar(kP + 2 * i + h), j & 1, abort_flag, err, kWaitCycles));
-            if (!ok) break;
-            tc_fence_after();
+        for (int h = 0; ok && h < 2; ++h) {
+          ok = __all_sync(0xffffffffu, mbar_wait(bar(kP + 2 * i + h), j & 1, abort_flag, err, kWaitCycles));
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              umma_lead_ta(leader, u_tmem + C::O_COL + i * HDP, u_tmem + i * 128 + h * 64 + ks * 8, umma_desc_sw128_n(v + (4 * h + ks) * 2048, 16384), kIdO,
-                           j > 0 || h > 0 || ks > 0);
-            commit_lead(leader, bar(kO + 2 * i + h));
-            const bool last = h == 1 && i == u_tiles - 1;
-            if (last) commit_lead(leader, bar(kEmpty + (2 * j + 1) % kRing));
-            if (j + 1 < u_nb) {
-              if (h == 0 && i == 0) {
-                ok = wait_tile(2 * j + 2);
-                if (!ok) break;
-                tc_fence_after();
-              }
-              scores(i, j + 1, h);
-              if (last) commit_lead(leader, bar(kEmpty + (2 * j + 2) % kRing));
+          for (int ks = 0; ks < 4; ++ks)
+            umma_lead_ta(leader, u_o, u_s + h * 64 + ks * 8, umma_desc_sw128_n(v + (4 * h + ks) * 2048, 16384), kIdO, j > 0 || h > 0 || ks > 0);
+          commit_lead(leader, bar(kO + 2 * i + h));
+          if (h) commit_lead(leader, bar(kEmpty + (2 * j + 1) % kRing));
+          if (j + 1 < u_nb) {
+            if (!h) {
+              ok = wait_tile(2 * j + 2);
+              if (!ok) break;
+              tc_fence_after();
             }
+            scores(j + 1, h);
+            if (h) commit_lead(leader, bar(kEmpty + (2 * j + 2) % kRing));
           }
+        }
       }
       // everything issued is done before the tensor memory goes back
-      commit_lead(leader, bar(kDrain));
-      mbar_wait(bar(kDrain), 0, nullptr, err, kWaitCycles);
+      commit_lead(leader, bar(kDrain + i));
+      mbar_wait(bar(kDrain + i), 0, nullptr, err, kWaitCycles);
     }
     __syncwarp();
     } else if (warp == C::SOFT + 1) {
@@ -505,7 +506,7 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
       // given up: this block's copies must land before its shared memory goes back
       for (int i = max(0, u - kRing); i < u; ++i) mbar_wait(bar(kFull + i % kRing), (i / kRing) & 1, nullptr, err, kWaitCycles);
     }
-    } else if (warp == C::SOFT + 2) {
+    } else if (warp == C::SOFT + 3) {
       chunk_end(a);  // the block ends after this warp
     }
   }
