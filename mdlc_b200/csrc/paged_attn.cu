@@ -16,6 +16,8 @@
 //     over the blocks whatever the requests' lengths; a tile cut between blocks leaves
 //     partial sums in the workspace, which the last of them to arrive adds in block order.
 //   chunk mode (many rows): a block per row tile, or several that share its keys.
+#include <climits>
+
 #include "func_attr.h"
 #include "paged_attn.cuh"
 
@@ -24,6 +26,7 @@ namespace {
 
 constexpr int kAttnThreads = 128;
 constexpr int kStages = 3;
+constexpr int kHiddenPage = INT_MIN;  // stands for a page that no row sees; an id of that value counts as the next one, no page either
 constexpr int kUnit = 128;      // keys of one unit of split work
 // What beginning and ending a tile costs, in units: without it a block whose share is many short requests ends long after
 // the others (64 requests of 64 to 8192 keys: the last SM 271k cycles, the mean 189k)
@@ -141,16 +144,18 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
     }
 
   auto base_of = [&](int blk) { return key_of_block(sp, blk, BT); };
-  // cache row (key `lane` of the block) or -1: hidden from every row, or no such page
-  auto row_of = [&](int blk) {
+  // page id of key `lane` of the block, kHiddenPage: hidden from every row. Loads only, so that several are in flight.
+  auto id_of = [&](int blk) {
     const int j = base_of(blk) + lane;
-    int row = -1;
-    if (blk < blk1 && lane < BT && j < rq.kv_len && (j >= sp.lo || j < d.sinks)) {
-      const int id = __ldg(a.table + (long long)b * d.table_stride + j / d.page);
-      if ((unsigned)id < (unsigned)d.pages) row = (id * d.kv_heads + e) * d.page + j % d.page;
-      else record_error(err, MDLC_DEVERR_BOUNDS);
-    }
-    return row;
+    if (blk >= blk1 || lane >= BT || j >= rq.kv_len || (j < sp.lo && j >= d.sinks)) return kHiddenPage;
+    return max(__ldg(a.table + (long long)b * d.table_stride + j / d.page), kHiddenPage + 1);
+  };
+  // its cache row, or -1: hidden or missing
+  auto row_of = [&](int blk, int id) {
+    if (id == kHiddenPage) return -1;
+    if ((unsigned)id < (unsigned)d.pages) return (id * d.kv_heads + e) * d.page + (base_of(blk) + lane) % d.page;
+    record_error(err, MDLC_DEVERR_BOUNDS);
+    return -1;
   };
   auto issue = [&](int blk, int row, int stage) {
     if (blk < blk1) {
@@ -174,23 +179,20 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
   float o[HDP / 8][4] = {};
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
   // key group wn takes blocks blk0 + wn, blk0 + wn + WN, ...
-  int row_next = -1;
-  {
-    int stage = 0;
-    for (; stage < kStages - 1; ++stage) {
-      const int blk = blk0 + wn + stage * WN;
-      issue(blk, row_of(blk), stage);
-    }
-    row_next = row_of(blk0 + wn + stage * WN);
-  }
+  int ids[kStages];
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) ids[i] = id_of(blk0 + wn + i * WN);
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) issue(blk0 + wn + i * WN, row_of(blk0 + wn + i * WN, ids[i]), i);
+  int id_next = ids[kStages - 1];
   int stage = 0;
   for (int blk = blk0 + wn; blk < blk1; blk += WN) {
     cp_async_wait<kStages - 2>();
     sync_group();
     {
       const int ahead = blk + (kStages - 1) * WN;
-      issue(ahead, row_next, stage == 0 ? kStages - 1 : stage - 1);
-      row_next = row_of(ahead + WN);
+      issue(ahead, row_of(ahead, id_next), stage == 0 ? kStages - 1 : stage - 1);
+      id_next = id_of(ahead + WN);
     }
     const uint32_t ks_addr = ring + stage * K::STAGE, vs_addr = ks_addr + BT * PITCH;
     const uint32_t valid = valid_s[wn][stage];
@@ -577,6 +579,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
   unsigned char* ring_p = smem + warp * C::STAGES * 2 * C::TILE;
   const int box = min(d.page, BT), boxes = BT / box;       // keys of a TMA box, boxes of a block
   const int none = d.pages * d.kv_heads * d.page;          // a row past the maps: zeros
+  const int page_log2 = 31 - __clz(d.page);                // a power of two
   // this lane's box: keys or values, 64-column half, page
   const int my_page = lane % boxes, my_half = lane / boxes % HALVES, my_kv = lane / (boxes * HALVES);
   const bool mine = my_kv < 2;
@@ -602,13 +605,16 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
 #pragma unroll
       for (int i = 0; i < 2; ++i) pos[n][i] = 8 * n + 2 * t + i < rows ? shift + (8 * n + 2 * t + i) / a.group : -1;
     }
-    // cache row of this lane's box (a row past the maps: hidden or missing), and whether its page exists
-    auto row_of = [&](int blk) {
-      if (blk >= blk1 || !mine) return none;
+    // page id of this lane's box, kHiddenPage: hidden from every row. Loads only, so that several are in flight.
+    auto id_of = [&](int blk) {
       const int k0 = key_of_block(sp, blk, BT) + my_page * box;
-      if (k0 >= sp.hi || (k0 + box <= sp.lo && k0 >= d.sinks)) return none;
-      const int id = __ldg(a.table + (long long)b * d.table_stride + k0 / d.page);
-      if ((unsigned)id < (unsigned)d.pages) return (id * d.kv_heads + e) * d.page + k0 % d.page;
+      if (blk >= blk1 || !mine || k0 >= sp.hi || (k0 + box <= sp.lo && k0 >= d.sinks)) return kHiddenPage;
+      return max(__ldg(a.table + (long long)b * d.table_stride + (k0 >> page_log2)), kHiddenPage + 1);
+    };
+    // its cache row, or one past the maps: hidden or missing
+    auto row_of = [&](int blk, int id) {
+      if (id == kHiddenPage) return none;
+      if ((unsigned)id < (unsigned)d.pages) return (id * d.kv_heads + e) * d.page + ((key_of_block(sp, blk, BT) + my_page * box) & (d.page - 1));
       record_error(err, MDLC_DEVERR_BOUNDS);
       return none;
     };
@@ -633,16 +639,21 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
     // this warp takes blocks blk0 + warp, blk0 + warp + 4, ...; the stage of a use is its number modulo STAGES
     int st = used % C::STAGES;
     auto next_stage = [&](int s, int by) { return (s + by) % C::STAGES; };
-    for (int i = 0; i < C::STAGES - 1; ++i) issue(blk0 + warp + 4 * i, row_of(blk0 + warp + 4 * i), next_stage(st, i));
-    int row_next = row_of(blk0 + warp + 4 * (C::STAGES - 1));
+    int ids[C::STAGES];
+#pragma unroll
+    for (int i = 0; i < C::STAGES; ++i) ids[i] = id_of(blk0 + warp + 4 * i);
+#pragma unroll
+    for (int i = 0; i < C::STAGES - 1; ++i) issue(blk0 + warp + 4 * i, row_of(blk0 + warp + 4 * i, ids[i]), next_stage(st, i));
+    int id_next = ids[C::STAGES - 1];
     bool ok = true;
     for (int blk = blk0 + warp; blk < blk1; blk += 4) {
-      __syncwarp();  // every lane has read the stage that is filled next
-      issue(blk + 4 * (C::STAGES - 1), row_next, next_stage(st, C::STAGES - 1));
-      row_next = row_of(blk + 4 * C::STAGES);
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full_s[warp][st]), (used / C::STAGES) & 1, nullptr, err, 2 * kWaitLimitNs));
       if (!ok) break;
       ++used;
+      __syncwarp();  // every lane has read the stage that is filled next (the block before this one's)
+      const int ahead = blk + 4 * (C::STAGES - 1);
+      issue(ahead, row_of(ahead, id_next), next_stage(st, C::STAGES - 1));
+      id_next = id_of(ahead + 4);
       const uint32_t ks_addr = ring + st * 2 * C::TILE, vs_addr = ks_addr + C::TILE;
       const int base = key_of_block(sp, blk, BT);
       uint32_t have = 0;
@@ -891,7 +902,8 @@ Chunk chunk_of(const mdlc_attn_desc& d) {
   c.tc = attn_tc_fits(d) && (long long)d.tokens * group / attn_tc_rows(d.head_dim) + d.batch <= 65535;  // the tiles are its grid's y
   c.rows = c.tc ? attn_tc_rows(d.head_dim) : 64;
   c.tiles = (int)min((long long)d.tokens * group / c.rows + d.batch, (long long)INT32_MAX);
-  // blocks on an SM: two of one row tile, one of two; three of the mma.sync kernel's
+  // blocks on an SM: two of one row tile, one of two; three shares of the mma.sync kernel's (it holds two or three: fp32, five mixed
+  // requests, 86 us with three, 110 with two)
   const long long room = kChunkBlocks * (c.tc ? (c.rows == 128 ? 2 : 1) : 3) / ((long long)c.tiles * d.kv_heads);
   c.splits = (int)max(1ll, min(room, min(16ll, (long long)d.max_kv / kLeastKeys)));
   return c;

@@ -432,6 +432,33 @@ def test_paged_attn_no_such_page(dev, rng):
         np.testing.assert_allclose(got, (w / w.sum(1, keepdims=True)) @ vv, atol=1e-4)
 
 
+@pytest.mark.parametrize("bad", [12, -1, -2, -2 ** 31, 2 ** 31 - 1])
+@pytest.mark.parametrize("new", [1, 150])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_paged_attn_no_such_page_ids(dev, rng, dtype, new, bad):
+    """Every id outside the cache is recorded and its keys hidden, whatever its value, in every type and form."""
+    ctx, d, page, kv = dev.ctx, 64, 16, 190
+    (q, qv), (k, kval), (v, vval) = (store(rng.standard_normal(s), dtype) for s in ((new, d), (12, page, d), (12, page, d)))
+    table = np.arange(12, dtype=np.int32)[None].copy()
+    table[0, 3] = bad
+    desc = L.AttnDesc(batch=1, tokens=new, heads=1, kv_heads=1, head_dim=d, page=page, pages=12, table_stride=12, max_q=new, max_kv=kv,
+                      dtype=ET[dtype], scale=0.125, q_stride=d, out_stride=d)
+    out = dev.out((new, d), RAW[dtype])
+    ctx.paged_attn(desc, dev.put(q), dev.put(k), dev.put(v), dev.put(table), dev.put(np.array([0, new], np.int32)),
+                   dev.put(np.array([kv], np.int32)), out, 0, dev.out(L.paged_attn_workspace(desc), np.uint8))
+    with pytest.raises(L.MdlcError):
+        ctx.sync()
+    got = dev.floats(out, (new, d), dtype)
+    kk, vv = (x.reshape(-1, d)[:kv].astype(np.float64) for x in (kval, vval))
+    j, p = np.arange(kv)[None], (kv - new + np.arange(new))[:, None]
+    s = np.where((j <= p) & (j // page != 3), 0.125 * (qv.astype(np.float64) @ kk.T), -np.inf)
+    w = np.exp(s - s.max(1, keepdims=True))
+    qk = 0.125 * math.sqrt((qv.astype(np.float64) ** 2).sum(-1).max() * (kk ** 2).sum(-1).max())
+    eps = (d * 2.0 ** -21 if dtype == "f32" else d * 2.0 ** -23) * qk + 4 * U * qk
+    tol = ((2 * eps + 64 * U) if dtype == "f32" else (2.5 * H + 2 * eps)) * abs(vv).max()
+    assert abs(got - (w / w.sum(1, keepdims=True)) @ vv).max() <= tol
+
+
 def test_paged_attn_refuses(ctx):
     ok = dict(batch=2, tokens=4, heads=8, kv_heads=2, head_dim=64, page=16, pages=9, table_stride=4, max_q=2, max_kv=60, dtype=L.BF16,
               scale=0.1, q_stride=512, out_stride=512)
