@@ -66,12 +66,17 @@ MDLC_DEV void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint3
 // high part (a tf32 value) and the exact rest of an fp32 number
 MDLC_DEV uint32_t tf_hi(uint32_t x) { return x & 0xffffe000u; }
 MDLC_DEV uint32_t tf_lo(uint32_t x) { return __float_as_uint(__uint_as_float(x) - __uint_as_float(tf_hi(x))); }
-// a b of fp32 operands in three tf32 products: c takes the large one, r the two small ones (sums of their own: shorter chains
-// of dependent products, and the truncation of one does not cut the other)
-MDLC_DEV void mma_3tf32(float (&c)[4], float (&r)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], uint32_t b0, uint32_t b1) {
-  mma_tf32(c, hi, tf_hi(b0), tf_hi(b1));
-  mma_tf32(r, lo, tf_hi(b0), tf_hi(b1));
-  mma_tf32(r, hi, tf_lo(b0), tf_lo(b1));
+// a b of fp32 operands in three tf32 products, for N accumulators at once: c takes the large one, r the two small ones (a sum
+// of its own: the truncation of one does not cut the other). All N products of a kind come before the next kind, so that a
+// product does not wait for the one before it (64 fp32 decodes of 4000 keys: 191 us; each accumulator's three in a row 208).
+template <int N>
+MDLC_DEV void mma_3tf32(float (*c)[4], float (*r)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], const uint32_t (&b)[N][2]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n) mma_tf32(r[n], lo, tf_hi(b[n][0]), tf_hi(b[n][1]));
+#pragma unroll
+  for (int n = 0; n < N; ++n) mma_tf32(c[n], hi, tf_hi(b[n][0]), tf_hi(b[n][1]));
+#pragma unroll
+  for (int n = 0; n < N; ++n) mma_tf32(r[n], hi, tf_lo(b[n][0]), tf_lo(b[n][1]));
 }
 
 MDLC_DEV void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -201,35 +206,37 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
     // scores
     float s[BT / 8][4] = {};
     constexpr int ST = kBf16 ? 1 : BT / 8;
-    float s_odd[ST][4] = {}, s_low[ST][4] = {};  // fp32: odd steps' products and the small ones
+    float s_low[ST][4] = {};  // fp32: the small products
     {
       const int mi = lane >> 3, r = lane & 7;
       const int key = (mi >> 1) * 8 + r;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t kb[BT / 8][2];
 #pragma unroll
         for (int nt = 0; nt < BT / 8; nt += 2) {
-          uint32_t kb[4];
-          ldsm_x4(kb, ks_addr + (nt * 8 + key) * PITCH + (((2 * ks + (mi & 1)) ^ r) << 4));
-          if constexpr (kBf16) {
-            mma_bf16(s[nt], qa[ks], kb[0], kb[1]);
-            mma_bf16(s[nt + 1], qa[ks], kb[2], kb[3]);
-          } else {
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              hi[i] = tf_hi(qa[ks][i]);
-              lo[i] = tf_lo(qa[ks][i]);
-            }
-            mma_3tf32(ks & 1 ? s_odd[nt] : s[nt], s_low[nt], hi, lo, kb[0], kb[1]);
-            mma_3tf32(ks & 1 ? s_odd[nt + 1] : s[nt + 1], s_low[nt + 1], hi, lo, kb[2], kb[3]);
-          }
+          uint32_t x[4];
+          ldsm_x4(x, ks_addr + (nt * 8 + key) * PITCH + (((2 * ks + (mi & 1)) ^ r) << 4));
+          kb[nt][0] = x[0], kb[nt][1] = x[1], kb[nt + 1][0] = x[2], kb[nt + 1][1] = x[3];
         }
+        if constexpr (kBf16) {
+#pragma unroll
+          for (int nt = 0; nt < BT / 8; ++nt) mma_bf16(s[nt], qa[ks], kb[nt][0], kb[nt][1]);
+        } else {
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            hi[i] = tf_hi(qa[ks][i]);
+            lo[i] = tf_lo(qa[ks][i]);
+          }
+          mma_3tf32(s, s_low, hi, lo, kb);
+        }
+      }
       if constexpr (!kBf16) {
 #pragma unroll
         for (int nt = 0; nt < BT / 8; ++nt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) s[nt][i] += s_odd[nt][i] + s_low[nt][i];
+          for (int i = 0; i < 4; ++i) s[nt][i] += s_low[nt][i];
       }
     }
     // mask, running maximum. A block that every row sees whole (all but the span's ends) needs no mask.
@@ -303,18 +310,25 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
           lo[kt][i] = tf_lo(x);
         }
       const int k0 = 2 * t, k1 = 2 * t + 1;
+      constexpr int ND = 4;  // tiles of 8 columns at once
 #pragma unroll
-      for (int nd = 0; nd < HDP / 8; ++nd) {
-        const int c = nd * 2 + (g >> 2);
-        float add[2][4] = {}, low[4] = {};
+      for (int nd = 0; nd < HDP / 8; nd += ND) {
+        float add[ND][4] = {}, low[ND][4] = {};
 #pragma unroll
         for (int kt = 0; kt < BT / 8; ++kt) {
-          const uint32_t b0 = lds32(vs_addr + (kt * 8 + k0) * PITCH + ((c ^ k0) << 4) + (g & 3) * 4);
-          const uint32_t b1 = lds32(vs_addr + (kt * 8 + k1) * PITCH + ((c ^ k1) << 4) + (g & 3) * 4);
-          mma_3tf32(add[kt & 1], low, hi[kt], lo[kt], b0, b1);
+          uint32_t vb[ND][2];
+#pragma unroll
+          for (int i = 0; i < ND; ++i) {
+            const int c = (nd + i) * 2 + (g >> 2);
+            vb[i][0] = lds32(vs_addr + (kt * 8 + k0) * PITCH + ((c ^ k0) << 4) + (g & 3) * 4);
+            vb[i][1] = lds32(vs_addr + (kt * 8 + k1) * PITCH + ((c ^ k1) << 4) + (g & 3) * 4);
+          }
+          mma_3tf32(add, low, hi[kt], lo[kt], vb);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[nd][i] += (add[0][i] + add[1][i]) + low[i];
+        for (int i = 0; i < ND; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[nd + i][j] += add[i][j] + low[i][j];
       }
     }
     stage = stage + 1 == kStages ? 0 : stage + 1;
@@ -814,7 +828,8 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
   split_walk<BT>(a, piece, [&](int b, const Request& rq, int e, int c0, int c1) { join_pieces<__nv_bfloat16, HDP, C::ROWS>(a, b, e, rq, c0, c1); });
 }
 
-// a block per row tile (x), key head (y) and share of its keys (z)
+// A block per row tile, share of its keys and key head, heads fastest: blocks start in this order and the tiles come with the
+// longest first, so the last to start are short (fp32, three prompts of up to 2000 tokens: 469 us, 584 with tiles fastest).
 template <typename T, int HDP>
 __global__ void __launch_bounds__(kAttnThreads) attn_chunk_kernel(const AttnArgs a, int* err) {
   using K = Cfg<T, HDP, 4>;
@@ -823,14 +838,14 @@ __global__ void __launch_bounds__(kAttnThreads) attn_chunk_kernel(const AttnArgs
   __shared__ long long warp_sums[kAttnThreads / 32];
   __shared__ Place place_s;
   chunk_begin(a);
+  const int e = blockIdx.x % a.d.kv_heads, tile = blockIdx.x / a.d.kv_heads / a.splits, z = blockIdx.x / a.d.kv_heads % a.splits;
   Tile t;
-  if (!find_tile(a, blockIdx.x, K::ROWS, warp_sums, &place_s, &t)) return chunk_end(a);
+  if (!find_tile(a, tile, K::ROWS, warp_sums, &place_s, &t)) return chunk_end(a);
   const Span sp = span_of(a, t.rq, t.r0 / a.group, (min(t.r0 + K::ROWS, t.rows) - 1) / a.group, K::BT);
-  const int ns = splits_of(a, sp.n, kLeastKeys / K::BT), z = blockIdx.z;
+  const int ns = splits_of(a, sp.n, kLeastKeys / K::BT);
   if (z >= ns) return;
-  attn_piece<T, HDP, 4>(a, attn_smem, valid_s, err, t.b, t.rq, blockIdx.y, t.r0, sp, (int)((long long)z * sp.n / ns),
-                        (int)((long long)(z + 1) * sp.n / ns), ns == 1,
-                        ((long long)blockIdx.x * a.d.kv_heads + blockIdx.y) * a.splits + z);
+  attn_piece<T, HDP, 4>(a, attn_smem, valid_s, err, t.b, t.rq, e, t.r0, sp, (int)((long long)z * sp.n / ns),
+                        (int)((long long)(z + 1) * sp.n / ns), ns == 1, ((long long)tile * a.d.kv_heads + e) * a.splits + z);
   chunk_end(a);
 }
 
@@ -902,9 +917,10 @@ Chunk chunk_of(const mdlc_attn_desc& d) {
   c.tc = attn_tc_fits(d) && (long long)d.tokens * group / attn_tc_rows(d.head_dim) + d.batch <= 65535;  // the tiles are its grid's y
   c.rows = c.tc ? attn_tc_rows(d.head_dim) : 64;
   c.tiles = (int)min((long long)d.tokens * group / c.rows + d.batch, (long long)INT32_MAX);
-  // blocks on an SM: two of one row tile, one of two; three shares of the mma.sync kernel's (it holds two or three: fp32, five mixed
-  // requests, 86 us with three, 110 with two)
-  const long long room = kChunkBlocks * (c.tc ? (c.rows == 128 ? 2 : 1) : 3) / ((long long)c.tiles * d.kv_heads);
+  // blocks on an SM: two of one row tile, one of two. The mma.sync kernel's shares are made for four, of which two run at a time:
+  // `tiles` counts a part-filled tile more per request than there may be (fp32, five mixed requests: three 83 us, four 73, five
+  // 84; twelve requests of up to 130 tokens: four 74, five 58)
+  const long long room = kChunkBlocks * (c.tc ? (c.rows == 128 ? 2 : 1) : 4) / ((long long)c.tiles * d.kv_heads);
   c.splits = (int)max(1ll, min(room, min(16ll, (long long)d.max_kv / kLeastKeys)));
   return c;
 }
@@ -994,15 +1010,16 @@ cudaError_t run_attn(mdlc_ctx* ctx, AttnArgs& sa, AttnArgs& a) {  // split mode'
   if (e != cudaSuccess || !c.used) return e;
   a.splits = c.splits;
   a.beside = wm > 0;
-  const dim3 grid(c.tiles, a.d.kv_heads, c.splits);
   mdlc_note_launch(ctx);
   if (c.tc) {
-    e = attn_tc_launch(ctx, a, grid);
+    e = attn_tc_launch(ctx, a, dim3(c.tiles, a.d.kv_heads, c.splits));
   } else {
     const int smem = Cfg<T, HDP, 4>::SMEM;
     static SmemLimit seen;
     e = allow_smem(seen, ctx->device, attn_chunk_kernel<T, HDP>, smem);
-    if (e == cudaSuccess) e = launch_pdl(attn_chunk_kernel<T, HDP>, grid, dim3(kAttnThreads), smem, ctx->stream, a, ctx->d_err);
+    const long long blocks = (long long)c.tiles * a.d.kv_heads * c.splits;
+    if (e == cudaSuccess && blocks > INT32_MAX) e = cudaErrorInvalidConfiguration;
+    if (e == cudaSuccess) e = launch_pdl(attn_chunk_kernel<T, HDP>, dim3((unsigned)blocks), dim3(kAttnThreads), smem, ctx->stream, a, ctx->d_err);
   }
   if (e != cudaSuccess || c.splits == 1) return e;
   mdlc_note_launch(ctx);
