@@ -27,6 +27,7 @@ namespace {
 constexpr int kAttnThreads = 128;
 constexpr int kStages = 3;
 constexpr int kHiddenPage = INT_MIN;  // stands for a page that no row sees; an id of that value counts as the next one, no page either
+constexpr int kTwoBlocks = 112 * 1024;  // shared memory of a block of which two fit on an SM
 constexpr int kUnit = 128;      // keys of one unit of split work
 // What beginning and ending a tile costs, in units: without it a block whose share is many short requests ends long after
 // the others (64 requests of 64 to 8192 keys: the last SM 271k cycles, the mean 189k)
@@ -53,6 +54,12 @@ MDLC_DEV uint32_t lds32(uint32_t addr) {
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
   return v;
 }
+MDLC_DEV void lds128(uint32_t (&v)[4], uint32_t addr) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+MDLC_DEV void sts128(uint32_t addr, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
 MDLC_DEV void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -66,9 +73,17 @@ MDLC_DEV void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint3
 // high part (a tf32 value) and the exact rest of an fp32 number
 MDLC_DEV uint32_t tf_hi(uint32_t x) { return x & 0xffffe000u; }
 MDLC_DEV uint32_t tf_lo(uint32_t x) { return __float_as_uint(__uint_as_float(x) - __uint_as_float(tf_hi(x))); }
+// the same with the high part rounded to the nearest, for the queries: their rests then have either sign, and so has the product of
+// two rests, which is dropped (an output error of 6.5e-7 over 1700 keys, 1.03e-6 without; one more integer addition each, which
+// weights take 3% longer for and 6e-8 closer)
+MDLC_DEV void tf_split(uint32_t x, uint32_t& hi, uint32_t& lo) {
+  hi = (x + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi));
+}
 // a b of fp32 operands in three tf32 products, for N accumulators at once: c takes the large one, r the two small ones (a sum
 // of its own: the truncation of one does not cut the other). All N products of a kind come before the next kind, so that a
-// product does not wait for the one before it (64 fp32 decodes of 4000 keys: 191 us; each accumulator's three in a row 208).
+// product does not wait for the one before it (64 fp32 decodes of 4000 keys, all else as it was then: 191 us; each accumulator's three
+// in a row 208).
 template <int N>
 MDLC_DEV void mma_3tf32(float (*c)[4], float (*r)[4], const uint32_t (&hi)[4], const uint32_t (&lo)[4], const uint32_t (&b)[N][2]) {
 #pragma unroll
@@ -100,7 +115,11 @@ struct Cfg {
   static constexpr int STAGE = 2 * BT * PITCH;             // keys and values of one block
   static constexpr int RING = WN * kStages * STAGE;
   static constexpr int MERGE = WN * ROWS * (HDP + 2) * 4;  // the key groups' sums, over the ring
-  static constexpr int SMEM = (RING > MERGE ? RING : MERGE);
+  // fp32 heads of more than 64 columns: the queries' high and low parts behind it, fragment by fragment, since 64 registers for them
+  // are too many (64 decodes of 4000 keys: 164 us, 192 from registers; heads of up to 64 columns: 98 us, 91 from registers)
+  static constexpr int QAT = (RING > MERGE ? RING : MERGE);
+  static constexpr bool QSHARED = sizeof(T) == 4 && HDP == 128;
+  static constexpr int SMEM = QAT + (QSHARED ? WM * (HDP / 8) * 1024 : 0);
 };
 
 // Rows [r0, r0 + 16 WM) of (request, key head e) over the span's blocks [blk0, blk1). Whole: writes out
@@ -148,6 +167,26 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
       qa[ks][i] = (qp[i & 1] && c < d.head_dim) ? __ldg(reinterpret_cast<const uint32_t*>(qp[i & 1] + c)) : 0u;
     }
 
+  // fp32: this lane's fragments of step ks, split. In shared memory each thread reads what it wrote itself.
+  const uint32_t q_at = smem_u32(smem) + K::QAT + wm * (HDP / 8) * 1024 + lane * 16;
+  if constexpr (K::QSHARED)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tf_split(qa[ks][i], hi[i], lo[i]);
+      sts128(q_at + ks * 1024, hi);
+      sts128(q_at + ks * 1024 + 512, lo);
+    }
+  auto query = [&](int ks, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    if constexpr (K::QSHARED) {
+      lds128(hi, q_at + ks * 1024);
+      lds128(lo, q_at + ks * 1024 + 512);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tf_split(qa[ks][i], hi[i], lo[i]);
+    }
+  };
   auto base_of = [&](int blk) { return key_of_block(sp, blk, BT); };
   // page id of key `lane` of the block, kHiddenPage: hidden from every row. Loads only, so that several are in flight.
   auto id_of = [&](int blk) {
@@ -206,8 +245,7 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
     // scores
     float s[BT / 8][4] = {};
     constexpr int ST = kBf16 ? 1 : BT / 8;
-    // fp32: odd steps' products and the small ones. Shorter chains of truncated additions: an output error of 1.03e-6 over 1700 keys
-    // against 1.19e-6 with one sum for even and odd steps (68.4 and 67.9 us)
+    // fp32: odd steps' products and the small ones: shorter chains of truncated additions (6.5e-7, 8.1e-7 without; 68.4 and 67.8 us)
     float s_odd[ST][4] = {}, s_low[ST][4] = {};
     {
       const int mi = lane >> 3, r = lane & 7;
@@ -226,11 +264,7 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
           for (int nt = 0; nt < BT / 8; ++nt) mma_bf16(s[nt], qa[ks], kb[nt][0], kb[nt][1]);
         } else {
           uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            hi[i] = tf_hi(qa[ks][i]);
-            lo[i] = tf_lo(qa[ks][i]);
-          }
+          query(ks, hi, lo);
           mma_3tf32(ks & 1 ? s_odd : s, s_low, hi, lo, kb);
         }
       }
@@ -273,8 +307,8 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
       }
     }
     // the tensor cores truncate the running sum at every addition, an error that grows with the number of
-    // keys: for fp32 each block is summed from zero and added with a rounded addition (over 1700 keys
-    // the error falls from 1.1e-5 to 1.03e-6; bf16 outputs do not show it)
+    // keys: for fp32 each block is summed from zero and added with a rounded addition (over 1700 keys,
+    // 1.1e-5 before this and the other measures, 6.5e-7 with them; bf16 outputs do not show it)
 #pragma unroll
     for (int nt = 0; nt < BT / 8; ++nt)
 #pragma unroll
@@ -969,7 +1003,7 @@ cudaError_t run_split(mdlc_ctx* ctx, const AttnArgs& a) {
   const cudaError_t e = allow_smem(seen, ctx->device, kern, smem);
   if (e != cudaSuccess) return e;
   // one or two blocks per SM, as shared memory allows
-  const int blocks = min(kMaxBlocks, ctx->num_sms * (smem <= 100 * 1024 ? 2 : 1));
+  const int blocks = min(kMaxBlocks, ctx->num_sms * (smem <= kTwoBlocks ? 2 : 1));
   mdlc_note_launch(ctx);
   return launch_pdl(kern, dim3(blocks), dim3(kAttnThreads), smem, ctx->stream, a, ctx->d_err);
 }
