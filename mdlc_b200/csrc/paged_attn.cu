@@ -954,8 +954,8 @@ Chunk chunk_of(const mdlc_attn_desc& d) {
   c.rows = c.tc ? attn_tc_rows(d.head_dim) : 64;
   c.tiles = (int)min((long long)d.tokens * group / c.rows + d.batch, (long long)INT32_MAX);
   // blocks on an SM: two of one row tile, one of two. The mma.sync kernel's shares are made for four, of which two run at a time:
-  // `tiles` counts a part-filled tile more per request than there may be (fp32, five mixed requests: three 83 us, four 73, five
-  // 84; twelve requests of up to 130 tokens: four 74, five 58)
+  // `tiles` counts a part-filled tile more per request than there may be (fp32, five mixed requests: four 68 us, five 75,
+  // eight 79; twelve requests of up to 130 tokens: four 74, five 58)
   const long long room = kChunkBlocks * (c.tc ? (c.rows == 128 ? 2 : 1) : 4) / ((long long)c.tiles * d.kv_heads);
   c.splits = (int)max(1ll, min(room, min(16ll, (long long)d.max_kv / kLeastKeys)));
   return c;
