@@ -27,7 +27,8 @@ namespace {
 constexpr int kAttnThreads = 128;
 constexpr int kStages = 3;
 constexpr int kHiddenPage = INT_MIN;  // stands for a page that no row sees; an id of that value counts as the next one, no page either
-constexpr int kTwoBlocks = 112 * 1024;  // shared memory of a block of which two fit on an SM
+constexpr int kSmShared = 224 * 1024;  // shared memory of an SM that blocks may ask for
+constexpr int kTwoBlocks = kSmShared / 2;  // shared memory of a block of which two fit on an SM
 constexpr int kUnit = 128;      // keys of one unit of split work
 // What beginning and ending a tile costs, in units: without it a block whose share is many short requests ends long after
 // the others (64 requests of 64 to 8192 keys: the last SM 271k cycles, the mean 189k)
@@ -873,16 +874,16 @@ __global__ void __launch_bounds__(kAttnThreads) attn_chunk_kernel(const AttnArgs
   __shared__ uint32_t valid_s[K::WN][kStages];
   __shared__ long long warp_sums[kAttnThreads / 32];
   __shared__ Place place_s;
-  chunk_begin(a);
+  pdl_wait();
+  pdl_trigger();
   const int e = blockIdx.x % a.d.kv_heads, tile = blockIdx.x / a.d.kv_heads / a.splits, z = blockIdx.x / a.d.kv_heads % a.splits;
   Tile t;
-  if (!find_tile(a, tile, K::ROWS, warp_sums, &place_s, &t)) return chunk_end(a);
+  if (!find_tile(a, tile, K::ROWS, warp_sums, &place_s, &t)) return;
   const Span sp = span_of(a, t.rq, t.r0 / a.group, (min(t.r0 + K::ROWS, t.rows) - 1) / a.group, K::BT);
   const int ns = splits_of(a, sp.n, kLeastKeys / K::BT);
   if (z >= ns) return;
   attn_piece<T, HDP, 4>(a, attn_smem, valid_s, err, t.b, t.rq, e, t.r0, sp, (int)((long long)z * sp.n / ns),
                         (int)((long long)(z + 1) * sp.n / ns), ns == 1, ((long long)tile * a.d.kv_heads + e) * a.splits + z);
-  chunk_end(a);
 }
 
 // Adds the shares of a chunk tile, in order. A warp per row.
@@ -1009,7 +1010,7 @@ cudaError_t run_split(mdlc_ctx* ctx, const AttnArgs& a) {
 }
 
 template <int HDP, int NT>
-cudaError_t run_narrow(mdlc_ctx* ctx, const AttnArgs& a, bool chunks) {
+cudaError_t run_narrow(mdlc_ctx* ctx, const AttnArgs& a, int beside) {  // shared memory of a chunk block that runs beside, 0: none does
   using C = NarrowCfg<HDP, NT>;
   CUtensorMap maps[2];
   cudaError_t e = attn_tensor_maps(a, min(a.d.page, C::BT), &maps[0], &maps[1]);
@@ -1017,8 +1018,10 @@ cudaError_t run_narrow(mdlc_ctx* ctx, const AttnArgs& a, bool chunks) {
   static SmemLimit seen;
   e = allow_smem(seen, ctx->device, attn_narrow_kernel<HDP, NT>, C::SMEM);
   if (e != cudaSuccess) return e;
-  // two blocks per SM; one where chunks of the same call run beside
-  const int blocks = min(kMaxBlocks, ctx->num_sms * (C::SMEM <= 100 * 1024 && !chunks ? 2 : 1));
+  // Two blocks per SM; one where that leaves room for a chunk block of the same call. Chunk blocks of wide heads fit beside neither one
+  // nor two (40 decodes of up to 8000 keys and 20 chunks of up to 400 tokens, 128-column heads: two 324 us, one 352).
+  const bool room = beside > 0 && C::SMEM + beside <= kSmShared;
+  const int blocks = min(kMaxBlocks, ctx->num_sms * (room ? 1 : 2));
   mdlc_note_launch(ctx);
   return launch_pdl(attn_narrow_kernel<HDP, NT>, dim3(blocks), dim3(kAttnThreads), C::SMEM, ctx->stream, a, maps[0], maps[1], ctx->d_err);
 }
@@ -1027,15 +1030,41 @@ cudaError_t run_narrow(mdlc_ctx* ctx, const AttnArgs& a, bool chunks) {
 bool narrow_fits(const mdlc_attn_desc& d) { return d.dtype == MDLC_BF16 && d.page >= 8 && (d.page & (d.page - 1)) == 0; }
 
 template <typename T, int HDP>
+cudaError_t run_chunks(mdlc_ctx* ctx, cudaStream_t stream, AttnArgs& a, const Chunk& c) {
+  a.splits = c.splits;
+  mdlc_note_launch(ctx);
+  cudaError_t e;
+  if (c.tc) {
+    e = attn_tc_launch(ctx, stream, a, dim3(c.tiles, a.d.kv_heads, c.splits));
+  } else {
+    const int smem = Cfg<T, HDP, 4>::SMEM;
+    static SmemLimit seen;
+    e = allow_smem(seen, ctx->device, attn_chunk_kernel<T, HDP>, smem);
+    const long long blocks = (long long)c.tiles * a.d.kv_heads * c.splits;
+    if (e == cudaSuccess && blocks > INT32_MAX) e = cudaErrorInvalidConfiguration;
+    if (e == cudaSuccess) e = launch_pdl(attn_chunk_kernel<T, HDP>, dim3((unsigned)blocks), dim3(kAttnThreads), smem, stream, a, ctx->d_err);
+  }
+  if (e != cudaSuccess || c.splits == 1) return e;
+  mdlc_note_launch(ctx);
+  return launch_pdl(attn_chunk_join_kernel<T, HDP>, dim3(c.tiles, a.d.kv_heads, c.rows / 16), dim3(kJoinThreads), 0, stream, a, c.rows,
+                    c.tc ? kTcKeys : block_keys<T, HDP>());
+}
+
+template <typename T, int HDP>
 cudaError_t run_attn(mdlc_ctx* ctx, AttnArgs& sa, AttnArgs& a) {  // split mode's and chunk mode's arguments
   const int wm = split_groups(a.d);
   const Chunk c = chunk_of(a.d);
-  cudaError_t e = cudaSuccess;
+  if (wm == 0) return run_chunks<T, HDP>(ctx, ctx->stream, a, c);
+  // Both modes in one call touch different rows and parts of the workspace: chunk mode goes to the side stream, which waits for
+  // the work before the call, and the compute stream for it (24 mixed requests of 64-column heads: 55.6 us, 62.1 one after the other).
+  cudaError_t e = c.used ? mdlc_fork(ctx) : cudaSuccess;
+  if (e != cudaSuccess) return e;
   if (wm == 1 && narrow_fits(a.d)) {
     // requests of up to 8 rows in one column tile; with more than 8 heads per key head, or several tokens, two
     const bool one = a.group <= 8 && ((long long)a.d.max_q * a.group <= 8 || (long long)a.d.max_q * a.group > 16);
     if (one) sa.split_rows = a.split_rows = 8;
-    e = one ? run_narrow<HDP, 1>(ctx, sa, c.used) : run_narrow<HDP, 2>(ctx, sa, c.used);
+    const int beside = c.used && c.tc ? attn_tc_smem(a.d.head_dim) : 0;
+    e = one ? run_narrow<HDP, 1>(ctx, sa, beside) : run_narrow<HDP, 2>(ctx, sa, beside);
   } else if (wm == 1) {
     e = run_split<T, HDP, 1>(ctx, sa);
   } else if (wm == 2) {
@@ -1043,24 +1072,10 @@ cudaError_t run_attn(mdlc_ctx* ctx, AttnArgs& sa, AttnArgs& a) {  // split mode'
   } else if (wm == 4) {
     e = run_split<T, HDP, 4>(ctx, sa);
   }
-  if (e != cudaSuccess || !c.used) return e;
-  a.splits = c.splits;
-  a.beside = wm > 0;
-  mdlc_note_launch(ctx);
-  if (c.tc) {
-    e = attn_tc_launch(ctx, a, dim3(c.tiles, a.d.kv_heads, c.splits));
-  } else {
-    const int smem = Cfg<T, HDP, 4>::SMEM;
-    static SmemLimit seen;
-    e = allow_smem(seen, ctx->device, attn_chunk_kernel<T, HDP>, smem);
-    const long long blocks = (long long)c.tiles * a.d.kv_heads * c.splits;
-    if (e == cudaSuccess && blocks > INT32_MAX) e = cudaErrorInvalidConfiguration;
-    if (e == cudaSuccess) e = launch_pdl(attn_chunk_kernel<T, HDP>, dim3((unsigned)blocks), dim3(kAttnThreads), smem, ctx->stream, a, ctx->d_err);
-  }
-  if (e != cudaSuccess || c.splits == 1) return e;
-  mdlc_note_launch(ctx);
-  return launch_pdl(attn_chunk_join_kernel<T, HDP>, dim3(c.tiles, a.d.kv_heads, c.rows / 16), dim3(kJoinThreads), 0, ctx->stream, a, c.rows,
-                    c.tc ? kTcKeys : block_keys<T, HDP>());
+  if (!c.used) return e;
+  if (e == cudaSuccess) e = run_chunks<T, HDP>(ctx, ctx->side_stream, a, c);
+  const cudaError_t joined = mdlc_join(ctx);
+  return e != cudaSuccess ? e : joined;
 }
 
 }  // namespace

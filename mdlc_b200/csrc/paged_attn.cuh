@@ -24,7 +24,6 @@ struct AttnArgs {
   SmallDiv group_div;
   int split_rows;     // requests with at most this many rows go to split mode
   int splits;         // chunk mode: blocks that may share a row tile's keys
-  int beside;         // chunk mode: runs beside the split kernel in front of it, see chunk_begin
   float scale_log2;   // scale * log2(e)
   // workspace: partial sums [slot][rows][hdp], their maxima (base-2 exponent) and sums [slot][rows]
   float *part_o, *part_m, *part_l;
@@ -35,7 +34,8 @@ struct AttnArgs {
 constexpr int kTcKeys = 128;
 int attn_tc_rows(int head_dim);
 bool attn_tc_fits(const mdlc_attn_desc& d);
-cudaError_t attn_tc_launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid);
+int attn_tc_smem(int head_dim);
+cudaError_t attn_tc_launch(mdlc_ctx* ctx, cudaStream_t stream, const AttnArgs& a, dim3 grid);
 // tensor maps of the two caches (rows of head_dim elements) with boxes of `box` rows x 64 columns, 128-byte swizzle
 cudaError_t attn_tensor_maps(const AttnArgs& a, int box, CUtensorMap* k, CUtensorMap* v);
 
@@ -136,18 +136,6 @@ MDLC_DEV bool find_tile(const AttnArgs& a, long long want, int tile_rows, long l
   t->rows = t->rq.q_len * a.group;
   return true;
 }
-// Chunk mode after split mode in one call: the two touch different rows and parts of the workspace, so a chunk block need
-// not wait for the split kernel to end. It starts once every split block has let dependents go, which they do
-// after their own wait, so all work before the call is done and visible. The kernel after this one waits for this one alone:
-// one block therefore waits for the split kernel before it ends.
-MDLC_DEV void chunk_begin(const AttnArgs& a) {
-  if (!a.beside) pdl_wait();
-  pdl_trigger();
-}
-MDLC_DEV void chunk_end(const AttnArgs& a) {
-  if (a.beside && (blockIdx.x | blockIdx.y | blockIdx.z) == 0) pdl_wait();
-}
-
 // blocks that share a tile of n key blocks: each gets at least two
 MDLC_DEV int splits_of(const AttnArgs& a, int n, int least) { return max(1, min(a.splits, n / least)); }
 

@@ -184,13 +184,14 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
     abort_s = missing_s = 0;
     fence_mbar_init();
   }
-  chunk_begin(a);
+  pdl_wait();
+  pdl_trigger();
   Tile t;
-  if (!find_tile(a, blockIdx.y, C::ROWS, warp_sums, &place_s, &t)) return chunk_end(a);
+  if (!find_tile(a, blockIdx.y, C::ROWS, warp_sums, &place_s, &t)) return;
   const int e = blockIdx.x;
   const Span sp = span_of(a, t.rq, t.r0 / a.group, (min(t.r0 + C::ROWS, t.rows) - 1) / a.group, kKeys);
   const int ns = splits_of(a, sp.n, 2);
-  if ((int)blockIdx.z >= ns) return;  // (the first share always has work)
+  if ((int)blockIdx.z >= ns) return;
   const int blk0 = (int)((long long)blockIdx.z * sp.n / ns), blk1 = (int)((long long)(blockIdx.z + 1) * sp.n / ns), nb = blk1 - blk0;
   const int shift = t.rq.kv_len - t.rq.q_len;
   const int n_tiles = C::TILES == 2 && t.rows - t.r0 > 128 ? 2 : 1;
@@ -526,8 +527,6 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
       // given up: this block's copies must land before its shared memory goes back
       for (int i = max(0, u - kRing); i < u; ++i) mbar_wait(bar(kFull + i % kRing), (i / kRing) & 1, nullptr, err, kWaitCycles);
     }
-    } else if (warp == C::SOFT + 3) {
-      chunk_end(a);  // the block ends after this warp
     }
   }
   __syncwarp();
@@ -538,7 +537,7 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
 }
 
 template <int HDP>
-cudaError_t launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid) {
+cudaError_t launch(mdlc_ctx* ctx, cudaStream_t stream, const AttnArgs& a, dim3 grid) {
   CUtensorMap maps[2];
   cudaError_t e = attn_tensor_maps(a, min(a.d.page, kKeys), &maps[0], &maps[1]);
   if (e != cudaSuccess) return e;
@@ -546,7 +545,7 @@ cudaError_t launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid) {
   e = allow_smem(seen, ctx->device, attn_tc_kernel<HDP>, TcCfg<HDP>::SMEM);
   if (e != cudaSuccess) return e;
   // key heads fastest: the tiles that see the most keys start first in all of them
-  return launch_pdl(attn_tc_kernel<HDP>, dim3(grid.y, grid.x, grid.z), dim3(TcCfg<HDP>::THREADS), TcCfg<HDP>::SMEM, ctx->stream, a, maps[0], maps[1], ctx->d_err);
+  return launch_pdl(attn_tc_kernel<HDP>, dim3(grid.y, grid.x, grid.z), dim3(TcCfg<HDP>::THREADS), TcCfg<HDP>::SMEM, stream, a, maps[0], maps[1], ctx->d_err);
 }
 
 }  // namespace
@@ -572,8 +571,10 @@ bool attn_tc_fits(const mdlc_attn_desc& d) {
 
 int attn_tc_rows(int head_dim) { return head_dim <= 64 ? TcCfg<64>::ROWS : TcCfg<128>::ROWS; }
 
-cudaError_t attn_tc_launch(mdlc_ctx* ctx, const AttnArgs& a, dim3 grid) {
-  return a.d.head_dim <= 64 ? launch<64>(ctx, a, grid) : launch<128>(ctx, a, grid);
+int attn_tc_smem(int head_dim) { return head_dim <= 64 ? TcCfg<64>::SMEM : TcCfg<128>::SMEM; }
+
+cudaError_t attn_tc_launch(mdlc_ctx* ctx, cudaStream_t stream, const AttnArgs& a, dim3 grid) {
+  return a.d.head_dim <= 64 ? launch<64>(ctx, stream, a, grid) : launch<128>(ctx, stream, a, grid);
 }
 
 }  // namespace mdlc

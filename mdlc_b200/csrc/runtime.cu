@@ -29,6 +29,16 @@ int mdlc_cuda_status(mdlc_ctx* ctx, cudaError_t e, const char* what) {
   return mdlc_set_error(ctx, MDLC_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
+cudaError_t mdlc_fork(mdlc_ctx* ctx) {
+  const cudaError_t e = cudaEventRecord(ctx->forked, ctx->stream);
+  return e != cudaSuccess ? e : cudaStreamWaitEvent(ctx->side_stream, ctx->forked, 0);
+}
+
+cudaError_t mdlc_join(mdlc_ctx* ctx) {
+  const cudaError_t e = cudaEventRecord(ctx->joined, ctx->side_stream);
+  return e != cudaSuccess ? e : cudaStreamWaitEvent(ctx->stream, ctx->joined, 0);
+}
+
 extern "C" {
 
 int mdlc_version(void) { return 100; }
@@ -55,6 +65,9 @@ int mdlc_ctx_create(int device, mdlc_ctx** out) {
   ctx->num_sms = prop.multiProcessorCount;
   if (cudaStreamCreateWithFlags(&ctx->own_stream, cudaStreamNonBlocking) != cudaSuccess ||
       cudaEventCreateWithFlags(&ctx->order, cudaEventDisableTiming) != cudaSuccess ||
+      cudaStreamCreateWithFlags(&ctx->side_stream, cudaStreamNonBlocking) != cudaSuccess ||
+      cudaEventCreateWithFlags(&ctx->forked, cudaEventDisableTiming) != cudaSuccess ||
+      cudaEventCreateWithFlags(&ctx->joined, cudaEventDisableTiming) != cudaSuccess ||
       cudaStreamCreateWithFlags(&ctx->copy_stream, cudaStreamNonBlocking) != cudaSuccess ||
       cudaMalloc(&ctx->d_err, 256) != cudaSuccess ||
       cudaMemset(ctx->d_err, 0, 256) != cudaSuccess || cudaMalloc(&ctx->d_pad, 4096) != cudaSuccess ||
@@ -87,6 +100,7 @@ int mdlc_ctx_destroy(mdlc_ctx* ctx) {
   // a bound stream may be gone by now: wait for the device instead
   if (ctx->bound) cudaDeviceSynchronize();
   cudaStreamSynchronize(ctx->own_stream);
+  cudaStreamSynchronize(ctx->side_stream);
   if (ctx->copy_stream) cudaStreamSynchronize(ctx->copy_stream);
   if (ctx->graph_exec) cudaGraphExecDestroy(ctx->graph_exec);
   if (ctx->graph) cudaGraphDestroy(ctx->graph);
@@ -99,6 +113,9 @@ int mdlc_ctx_destroy(mdlc_ctx* ctx) {
   cudaFree(ctx->d_split_cnt);
   cudaFree(ctx->d_attn_cnt);
   cudaEventDestroy(ctx->order);
+  cudaEventDestroy(ctx->forked);
+  cudaEventDestroy(ctx->joined);
+  cudaStreamDestroy(ctx->side_stream);
   cudaStreamDestroy(ctx->own_stream);
   if (ctx->copy_stream) cudaStreamDestroy(ctx->copy_stream);
   delete ctx;

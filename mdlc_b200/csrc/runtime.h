@@ -20,6 +20,9 @@ struct mdlc_ctx {
   cudaStream_t own_stream = nullptr;
   bool bound = false;                  // stream is a caller's
   cudaEvent_t order = nullptr;         // orders the two when the binding changes
+  // work of one call that may run beside the rest of it (mdlc_fork / mdlc_join), with the events that order it
+  cudaStream_t side_stream = nullptr;
+  cudaEvent_t forked = nullptr, joined = nullptr;
   cudaStream_t copy_stream = nullptr;  // host<->device transfers overlapped with compute
   int* d_err = nullptr;  // device error word (first failure wins)
   uint8_t* d_pad = nullptr;  // 256 x 16-byte fill patterns (byte value v at v*16)
@@ -42,6 +45,10 @@ struct mdlc_ctx {
 
 int mdlc_set_error(mdlc_ctx* ctx, int status, const char* fmt, ...);
 int mdlc_cuda_status(mdlc_ctx* ctx, cudaError_t e, const char* what);
+// The side stream waits for what the compute stream has been given so far / the compute stream for the side stream. Every
+// fork is joined before its call returns, so a capture sees one stream again.
+cudaError_t mdlc_fork(mdlc_ctx* ctx);
+cudaError_t mdlc_join(mdlc_ctx* ctx);
 
 constexpr size_t kSplitWsBytes = 8u << 20;  // split-K partials: 64 units of 128 x 256 fp32
 constexpr int kSplitCounters = 1024;
