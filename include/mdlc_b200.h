@@ -461,8 +461,10 @@ int mdlc_rope_append(mdlc_ctx* ctx, const mdlc_rope_desc* desc, const void* q, c
  * optional, [tokens][heads] fp32, may be null). Table entries of pages that no new
  * token sees (behind the window, past kv_lens) are not read. A page id
  * outside [0, pages) among the read ones counts as hidden keys. Keys and values
- * past kv_lens may hold anything, NaN included; a non-finite one within it may reach
- * tokens that do not see it (as 0 x inf). Rows past q_starts[batch] are left
+ * past kv_lens may hold anything, NaN included. A NaN score makes its row's out
+ * and lse NaN, a score of +inf makes out NaN; in fp32 an infinite element of q, k or v
+ * counts as NaN. A non-finite value within kv_lens may reach tokens that do not see
+ * it (as 0 x inf). Rows past q_starts[batch] are left
  * as they are. `workspace`: mdlc_paged_attn_workspace bytes, 16-byte aligned, for
  * this call alone. q, out and caches are 16-byte aligned, the strides multiples of 8
  * elements. max_q and max_kv bound every request's q_len and kv_len: longer ones

@@ -42,8 +42,9 @@ struct TcCfg {
   // 2 x 128 x 208 + 128 x 88 = 384 x 168
   static constexpr int SOFT_REGS = TILES == 1 ? 168 : 208, OTHER_REGS = 88;
   // Of 16 pairs of weights, how many take 2^x on the fp32 pipe beside the special-function unit (16 a clock), which the two tiles'
-  // softmax share: 0.5 TFLOP of chunks 477 us with none, 454 with 4, 461 with 6; with one tile, none is as fast
-  static constexpr int POLY = TILES == 2 ? 4 : 0;
+  // softmax share: 0.5 TFLOP of chunks in short runs on a cool chip 464 us with 3, 474 with 4, 490 with 2; with one tile, none is
+  // as fast
+  static constexpr int POLY = TILES == 2 ? 3 : 0;
   static constexpr int HALVES = HDP / 64;               // 128-byte wide column blocks
   static constexpr int TILE = 128 * HDP * 2;            // one Q tile, one key or value tile
   static constexpr int Q = 0;
@@ -133,19 +134,31 @@ MDLC_DEV float ex2(float x) {
   return y;
 }
 
+MDLC_DEV float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+MDLC_DEV float2 mul2(const float2 a, const float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
+  return f2_from(r);
+}
+
 // 2^x of two values on the fp32 pipe: x = n + f with n the nearest integer (added and taken off again at 1.5 x 2^23, where
-// fp32 numbers are the integers), 2^f on [-1/2, 1/2] by a polynomial of degree 4, n added to the exponent bits. The
+// fp32 numbers are the integers), 2^f on [-1/2, 1/2] by a polynomial of degree 4, times 2^n made from n's bits. The
 // coefficients are a fit of smallest maximal relative error on that interval (2.6e-6, far below the bf16 rounding of the
-// weights). x below -126 gives a number near 2^-126, which the caller makes harmless, instead of 0.
+// weights). Numbers from -127 down are taken as -127, whose 2^n has the bits of 0: a hidden key (-inf) weighs exactly 0, and what is
+// below 2^-126.5 counts as 0 too. NaN stays NaN: the maximum passes it on, and the last step is a product.
 MDLC_DEV float2 ex2_poly(float2 x) {
-  x = make_float2(fmaxf(x.x, -126.0f), fmaxf(x.y, -126.0f));  // lower, the exponent of p would wrap
+  x = make_float2(max_nan(x.x, -127.0f), max_nan(x.y, -127.0f));
   const float2 t = add2(x, splat2(12582912.0f));
   const float2 f = fma2(add2(t, splat2(-12582912.0f)), splat2(-1.0f), x);
   float2 p = fma2(f, splat2(0.009570104070f), splat2(0.05591790378f));
   p = fma2(f, p, splat2(0.2402474582f));
   p = fma2(f, p, splat2(0.6931217909f));
   p = fma2(f, p, splat2(0.9999992847f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+  return mul2(p, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)));
 }
 
 template <int HDP>
@@ -366,7 +379,6 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
         tc_fence_before();
         mbar_arrive(bar(kP + 2 * tile + h));
       }
-      if (m == -INFINITY) l = 0.0f;  // no key seen: what is left are weights near 2^-126
       if (ok && nb > 0) ok = mbar_wait(bar(kO + 2 * tile + 1), (nb - 1) & 1, abort_flag, err, kWaitCycles);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
