@@ -409,6 +409,8 @@ int mdlc_se_fc(mdlc_ctx* ctx, const mdlc_se_desc* desc, const void* pooled, cons
  * q_starts[batch + 1]: running sums of new_lens, at most `tokens`; kv_lens[b]
  * = cached + new; slots[tokens], positions[tokens]: each new token's slot and its
  * index in its request; rows past the last request's get slot -1, position 0.
+ * A new token on a page whose id is negative or so large that its slot does not
+ * fit 32 bits gets slot -1 (and the error word MDLC_DEVERR_BOUNDS).
  * status[0]: pages taken from the list; status[1]: requests refused. Negative
  * lengths count as 0. Outputs must not overlap inputs; called again on the
  * same inputs it gives the same outputs. */

@@ -1,6 +1,8 @@
 // Bookkeeping of a paged key / value cache: mdlc_page_plan (block tables, slot
 // maps and positions from request lengths) and mdlc_rope_append (rotary
 // positions on queries and keys, keys and values written to their slots).
+#include <climits>
+
 #include "paged_attn.cuh"
 
 namespace mdlc {
@@ -49,7 +51,7 @@ MDLC_DEV uint32_t pages_of(uint32_t tok, const PageDiv& d) {
   return n + (n * d.page != tok);
 }
 
-__global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page_desc d, const PlanPtrs p, const PageDiv pd) {
+__global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page_desc d, const PlanPtrs p, const PageDiv pd, int* err) {
   pdl_wait();
   pdl_trigger();
   extern __shared__ int32_t plan_smem[];
@@ -152,7 +154,10 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page
         // a page taken by this call comes from the free list itself: its table entry may not be written yet
         const int id = at < held ? __ldg(p.table + (long long)lo * d.table_stride + at)
                                  : __ldg(p.free_list + first[lo] + (at - held));
-        if (id >= 0) slot = id * d.page + (pos - at * d.page);
+        // an id whose slots do not fit 32 bits would wrap onto another page's
+        const long long wide = (long long)id * d.page + (pos - at * d.page);
+        if (id >= 0 && wide <= INT_MAX) slot = (int)wide;
+        else record_error(err, MDLC_DEVERR_BOUNDS);
       }
     }
     p.slots[t] = slot;
@@ -367,7 +372,7 @@ extern "C" int mdlc_page_plan(mdlc_ctx* ctx, const mdlc_page_desc* d, const int3
   PageDiv pd = {(uint32_t)d->page, -1};
   for (int i = 0; i <= 10; ++i)
     if (d->page == 1 << i) pd.shift = i;
-  const cudaError_t e = launch_pdl(page_plan_kernel, dim3(blocks), dim3(kPlanThreads), smem, ctx->stream, *d, p, pd);
+  const cudaError_t e = launch_pdl(page_plan_kernel, dim3(blocks), dim3(kPlanThreads), smem, ctx->stream, *d, p, pd, ctx->d_err);
   mdlc_note_launch(ctx);
   return mdlc_cuda_status(ctx, e, "page_plan launch");
 }
