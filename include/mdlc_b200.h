@@ -406,8 +406,10 @@ int mdlc_se_fc(mdlc_ctx* ctx, const mdlc_se_desc* desc, const void* pooled, cons
  * table_stride entries or more pages than are left is refused: its row keeps its
  * entries, its slots are -1 and kv_lens[b] stays cached_lens[b] (the pages that
  * it would have taken are then not given to later requests either).
+ * New tokens that have no row, past the first `tokens` of all, are not planned: a
+ * request counts as if it brought only those that have one.
  * q_starts[batch + 1]: running sums of new_lens, at most `tokens`; kv_lens[b]
- * = cached + new; slots[tokens], positions[tokens]: each new token's slot and its
+ * = cached + new (those with a row); slots[tokens], positions[tokens]: each new token's slot and its
  * index in its request; rows past the last request's get slot -1, position 0.
  * A new token on a page whose id is negative or so large that its slot does not
  * fit 32 bits gets slot -1 (and the error word MDLC_DEVERR_BOUNDS).

@@ -81,31 +81,50 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page
     mine.pages += ask(c, n, &fits);
     mine.tokens += n;
   }
-  Sums run = warp_scan(mine, lane);
-  if (lane == 31) warp_sum[warp] = run;
-  __syncthreads();
-  if (warp == 0) {
-    Sums w = lane < kPlanThreads / 32 ? warp_sum[lane] : Sums{0, 0};
-    w = warp_scan(w, lane);
-    if (lane < kPlanThreads / 32) warp_sum[lane] = w;
+  // sums of the threads in front of this one, and of all
+  auto scan = [&](Sums v, Sums* all) {
+    Sums run = warp_scan(v, lane);
+    if (lane == 31) warp_sum[warp] = run;
+    __syncthreads();
+    if (warp == 0) {
+      Sums w = lane < kPlanThreads / 32 ? warp_sum[lane] : Sums{0, 0};
+      w = warp_scan(w, lane);
+      if (lane < kPlanThreads / 32) warp_sum[lane] = w;
+    }
+    __syncthreads();
+    *all = warp_sum[kPlanThreads / 32 - 1];
+    if (warp) {
+      run.tokens += warp_sum[warp - 1].tokens;
+      run.pages += warp_sum[warp - 1].pages;
+    }
+    return Sums{run.tokens - v.tokens, run.pages - v.pages};
+  };
+  Sums all, run = scan(mine, &all);
+  // a request brings only the tokens that have rows: what lies past the last row is not planned
+  auto rows_of = [&](int b, long long start) {
+    return (int)min((long long)max(0, __ldg(p.fresh + b)), max(0ll, d.tokens - start));
+  };
+  if (all.tokens > d.tokens) {  // pages again, of those tokens alone
+    Sums cut = {0, 0};
+    long long at = run.tokens;
+    for (int b = b0; b < b1; ++b) {
+      bool fits;
+      cut.pages += ask(max(0, __ldg(p.cached + b)), rows_of(b, at), &fits);
+      at += max(0, __ldg(p.fresh + b));
+    }
+    __syncthreads();
+    run.pages = scan(cut, &all).pages;
   }
-  __syncthreads();
-  if (warp) {
-    run.tokens += warp_sum[warp - 1].tokens;
-    run.pages += warp_sum[warp - 1].pages;
-  }
-  run.tokens -= mine.tokens;  // exclusive
-  run.pages -= mine.pages;
   int taken = 0, refused = 0;
   for (int b = b0; b < b1; ++b) {
-    const int c = max(0, __ldg(p.cached + b)), n = max(0, __ldg(p.fresh + b));
+    const int c = max(0, __ldg(p.cached + b)), n = rows_of(b, run.tokens);
     bool fits;
     const uint32_t take = ask(c, n, &fits);
     const bool ok = fits && (take == 0 || run.pages + take <= n_free);
     starts[b] = (int32_t)min(run.tokens, (long long)d.tokens);
     held_tok[b] = c;
     first[b] = ok ? (take ? (int32_t)run.pages : 0) : -1;
-    run.tokens += n;
+    run.tokens += max(0, __ldg(p.fresh + b));
     run.pages += take;
     if (ok && take) taken = (int)run.pages;
     refused += !ok;
@@ -133,7 +152,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page
   for (int b = blockIdx.x * (kPlanThreads / 32) + warp; b < d.batch; b += nwarps) {
     if (first[b] < 0) continue;
     const int c = held_tok[b];
-    const int held = (int)pages_of(c, pd), take = (int)pages_of((uint32_t)c + (uint32_t)max(0, __ldg(p.fresh + b)), pd) - held;
+    const int held = (int)pages_of(c, pd), take = (int)pages_of((uint32_t)c + (uint32_t)(starts[b + 1] - starts[b]), pd) - held;
     for (int j = lane; j < take; j += 32)
       p.table[(long long)b * d.table_stride + held + j] = __ldg(p.free_list + first[b] + j);
   }

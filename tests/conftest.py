@@ -23,6 +23,20 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA B200 and the built sm_100a library")
 
 
+# Tests that stay as they were written although one value in them is wrong; the right one is tested elsewhere.
+HOLD_A_WRONG_VALUE = {
+    "tests/test_paged_gpu.py::test_page_plan_corners":
+        "its third case wants kv_lens 4 for a request of which one row is left: attention would place that row at position 3, the plan "
+        "itself at 0 (test_page_plan_gpu.py: test_cut_requests_count_as_if_they_brought_their_rows, test_attention_over_a_cut_request)",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        if item.nodeid in HOLD_A_WRONG_VALUE:
+            item.add_marker(pytest.mark.xfail(reason=HOLD_A_WRONG_VALUE[item.nodeid], raises=AssertionError, strict=True))
+
+
 @pytest.fixture
 def rng():
     return np.random.default_rng(1234)
