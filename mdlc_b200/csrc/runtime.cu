@@ -199,32 +199,32 @@ int mdlc_memset(mdlc_ctx* ctx, void* dev, int value, size_t bytes) {
   return mdlc_cuda_status(ctx, cudaMemsetAsync(dev, value, bytes, ctx->stream), "memset");
 }
 
-static cudaStream_t stream_of(mdlc_ctx* ctx, int s) {
-  return s == MDLC_STREAM_COPY ? ctx->copy_stream : (s == MDLC_STREAM_COMPUTE ? ctx->stream : nullptr);
-}
+// (a null stream is a bound one's: the legacy default stream)
+static bool known_stream(int s) { return s == MDLC_STREAM_COPY || s == MDLC_STREAM_COMPUTE; }
+static cudaStream_t stream_of(mdlc_ctx* ctx, int s) { return s == MDLC_STREAM_COPY ? ctx->copy_stream : ctx->stream; }
 
 int mdlc_upload_on(mdlc_ctx* ctx, int stream, void* dev, const void* host, size_t bytes) {
-  if (!ctx || !stream_of(ctx, stream) || (!dev && bytes) || (!host && bytes)) return MDLC_ERR_INVALID;
+  if (!ctx || !known_stream(stream) || (!dev && bytes) || (!host && bytes)) return MDLC_ERR_INVALID;
   cudaSetDevice(ctx->device);
   return mdlc_cuda_status(
       ctx, cudaMemcpyAsync(dev, host, bytes, cudaMemcpyHostToDevice, stream_of(ctx, stream)), "upload");
 }
 
 int mdlc_download_on(mdlc_ctx* ctx, int stream, void* host, const void* dev, size_t bytes) {
-  if (!ctx || !stream_of(ctx, stream) || (!dev && bytes) || (!host && bytes)) return MDLC_ERR_INVALID;
+  if (!ctx || !known_stream(stream) || (!dev && bytes) || (!host && bytes)) return MDLC_ERR_INVALID;
   cudaSetDevice(ctx->device);
   return mdlc_cuda_status(
       ctx, cudaMemcpyAsync(host, dev, bytes, cudaMemcpyDeviceToHost, stream_of(ctx, stream)), "download");
 }
 
 int mdlc_fence_record(mdlc_ctx* ctx, int id, int stream) {
-  if (!ctx || id < 0 || id >= kMaxFences || !stream_of(ctx, stream)) return MDLC_ERR_INVALID;
+  if (!ctx || id < 0 || id >= kMaxFences || !known_stream(stream)) return MDLC_ERR_INVALID;
   cudaSetDevice(ctx->device);
   return mdlc_cuda_status(ctx, cudaEventRecord(ctx->fences[id], stream_of(ctx, stream)), "fence record");
 }
 
 int mdlc_fence_wait(mdlc_ctx* ctx, int id, int stream) {
-  if (!ctx || id < 0 || id >= kMaxFences || !stream_of(ctx, stream)) return MDLC_ERR_INVALID;
+  if (!ctx || id < 0 || id >= kMaxFences || !known_stream(stream)) return MDLC_ERR_INVALID;
   cudaSetDevice(ctx->device);
   return mdlc_cuda_status(ctx, cudaStreamWaitEvent(stream_of(ctx, stream), ctx->fences[id], 0), "fence wait");
 }
@@ -326,7 +326,7 @@ int mdlc_event_record(mdlc_ctx* ctx, int slot) {
 }
 
 int mdlc_event_record_on(mdlc_ctx* ctx, int slot, int stream) {
-  if (!ctx || slot < 0 || slot >= kMaxEvents || !stream_of(ctx, stream)) return MDLC_ERR_INVALID;
+  if (!ctx || slot < 0 || slot >= kMaxEvents || !known_stream(stream)) return MDLC_ERR_INVALID;
   cudaSetDevice(ctx->device);
   return mdlc_cuda_status(ctx, cudaEventRecord(ctx->events[slot], stream_of(ctx, stream)), "event record");
 }
