@@ -284,6 +284,7 @@ int mdlc_check_flag(mdlc_ctx* ctx, int* flag) {
 
 int mdlc_graph_begin(mdlc_ctx* ctx) {
   if (!ctx) return MDLC_ERR_INVALID;
+  if (ctx->capturing) return mdlc_set_error(ctx, MDLC_ERR_INVALID, "a capture is open already");
   cudaSetDevice(ctx->device);
   mdlc_graph_reset(ctx);
   // the legacy default stream (a bound one) cannot be captured: no capture is open then

@@ -58,3 +58,19 @@ def test_stream_ids_while_a_stream_is_bound(ctx, bound):
         with pytest.raises(L.MdlcError) as e:
             ctx.fence_record(3, bad)
         assert e.value.status == L.ERR_INVALID
+
+
+def test_a_second_begin_leaves_the_capture_open(ctx):
+    dev = ctx.alloc(256)
+    ctx.memset(dev, 0, 256)
+    ctx.graph_begin()
+    ctx.memset(dev, 7, 256)
+    with pytest.raises(L.MdlcError) as e:
+        ctx.graph_begin()
+    assert e.value.status == L.ERR_INVALID
+    ctx.graph_end()
+    ctx.graph_launch()
+    assert (ctx.download(dev, 256, np.uint8) == 7).all()
+    ctx.graph_reset()
+    with pytest.raises(L.MdlcError):
+        ctx.graph_end()
