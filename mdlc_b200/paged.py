@@ -119,7 +119,16 @@ class PagedCache:
             raise ValueError(f"a request would pass {self.max_len} tokens")
         if need.sum() > len(self.free):
             raise L.MdlcError(L.ERR_NOMEM, f"{int(need.sum())} pages wanted, {len(self.free)} free")
-        ctx, taken = self.ctx, int(need.sum())
+        ctx, taken, max_q = self.ctx, int(need.sum()), int(new.max())
+        # before anything is planned: a step that finds no memory leaves the cache as it was
+        room = L.paged_attn_workspace(self._attn(total, max_q))
+        if room > self._room:
+            ctx.sync()
+            old, self.workspace, self._room = self.workspace, 0, 0
+            if old:
+                ctx.free(old)
+            self.workspace = ctx.alloc(room)
+            self._room = room
         ctx.upload(self._cached, self.lens.astype(np.int32))
         ctx.upload(self._new, new.astype(np.int32))
         if taken:
@@ -128,13 +137,7 @@ class PagedCache:
         ctx.page_plan(desc, self._cached, self._new, self._free, 0, self.table, self.q_starts, self.kv_lens, self.slots, self.positions, self.status)
         del self.free[:taken]
         self.lens += new
-        self.tokens, self.max_q = total, int(new.max())
-        need = L.paged_attn_workspace(self._attn(total, self.max_q))
-        if need > self._room:
-            ctx.sync()
-            if self._room:
-                ctx.free(self.workspace)
-            self.workspace, self._room = ctx.alloc(need), need
+        self.tokens, self.max_q = total, max_q
 
     def append(self, layer: int, qkv: int, q_out: int) -> None:
         """Rotate the queries of the packed [tokens][heads + 2 kv_heads][head_dim] projection into ``q_out`` and write its

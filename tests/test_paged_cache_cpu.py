@@ -1,0 +1,78 @@
+"""The host side of a paged cache against a context that only keeps books (no GPU needed): what it allocates, gives back and
+uploads, and what is left of it when a call fails."""
+
+import numpy as np
+import pytest
+
+from mdlc_b200 import _lib as L
+from mdlc_b200 import paged
+
+
+class Books:
+    """Stands in for a Context: addresses that are handed out once, and a page plan after its definition."""
+
+    def __init__(self):
+        self.next, self.live, self.fail, self.plans, self.uploads = 1 << 20, {}, None, [], {}
+
+    def alloc(self, nbytes):
+        if self.fail is not None and nbytes >= self.fail:
+            raise L.MdlcError(L.ERR_NOMEM, "alloc")
+        self.next += 1 << 12
+        self.live[self.next] = nbytes
+        return self.next
+
+    def free(self, p):
+        del self.live[p]          # KeyError: not an allocation, or freed twice
+
+    def to_device(self, a):
+        p = self.alloc(a.nbytes)
+        self.uploads[p] = np.array(a)
+        return p
+
+    def upload(self, p, a):
+        assert a.nbytes <= self.live[p]
+        self.uploads[p] = np.array(a)
+
+    def download(self, p, shape, dtype):
+        raise AssertionError("a step reads nothing back")
+
+    def sync(self):
+        pass
+
+    def page_plan(self, desc, cached, new, free, count, table, *outs):
+        self.plans.append((self.uploads[cached].tolist(), self.uploads[new].tolist(),
+                           self.uploads[free].tolist()[:desc.free_pages] if desc.free_pages else []))
+
+    def rope_append(self, *a):
+        pass
+
+    def paged_attn(self, desc, q, k, v, table, q_starts, kv_lens, out, lse, workspace):
+        assert workspace in self.live and self.live[workspace] >= L.paged_attn_workspace(desc)
+
+    def gemv_w4(self, desc, x, codes, scales, zeros, bias, y):
+        assert codes in self.live and scales in self.live
+
+
+def cache(books, **kw):
+    args = dict(layers=1, batch=2, pages=40, page=4, heads=2, kv_heads=1, head_dim=8, max_tokens=64, max_len=64, dtype=L.F32)
+    return paged.PagedCache(books, **{**args, **kw})
+
+
+def test_workspace_that_cannot_grow():
+    """No memory for a larger workspace: the freed one is not used again, and lengths and pages are as before."""
+    b = Books()
+    c = cache(b, heads=8, kv_heads=1, head_dim=64, pages=600, max_tokens=300, max_len=2048)
+    c.plan([1, 1])
+    before = c._room
+    grown = L.paged_attn_workspace(c._attn(201, 200))
+    assert grown > before
+    b.fail = grown
+    lens, free = c.lens.copy(), list(c.free)
+    with pytest.raises(L.MdlcError):
+        c.plan([200, 1])
+    assert (c.lens == lens).all() and c.free == free and len(b.plans) == 1
+    b.fail = None
+    c.plan([1, 1])                # needs no more than the one that is gone
+    c.attend(0, 1, 2)             # checks that its workspace is allocated
+    c.close()
+    assert not b.live
