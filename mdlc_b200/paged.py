@@ -157,6 +157,8 @@ class PagedCache:
 
     def release(self, place: int) -> None:
         """End the request at ``place``: its pages go back to the free list."""
+        if not 0 <= place < self.batch:
+            raise ValueError(f"place {place} of {self.batch}")
         held = -(-int(self.lens[place]) // self.page)
         if held:
             ids = self.ctx.download(self.table + 4 * place * self.stride, (held,), np.int32)

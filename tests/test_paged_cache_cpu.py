@@ -76,3 +76,14 @@ def test_workspace_that_cannot_grow():
     c.attend(0, 1, 2)             # checks that its workspace is allocated
     c.close()
     assert not b.live
+
+
+@pytest.mark.parametrize("place", [-1, -2, 2, 100])
+def test_release_of_no_such_place(place):
+    """Refused: a negative place would read in front of the block table."""
+    b = Books()
+    c = cache(b)
+    c.plan([5, 6])
+    with pytest.raises(ValueError):
+        c.release(place)
+    assert list(c.lens) == [5, 6] and len(c.free) == 40 - 4
