@@ -4,7 +4,7 @@ decoder with their page bookkeeping, 4-bit weights, and rotation tables.
 A step of a decoder is one :meth:`PagedCache.plan` (block tables, slots and positions
 built on the GPU), then per layer :class:`W4Linear` projections, :meth:`PagedCache.append`
 (rotation and cache write) and :meth:`PagedCache.attend`. The kernels are asynchronous on the
-context's stream; ``plan`` uploads the step's lengths and ``release`` reads a table row, which wait for it.
+context's stream; ``plan`` uploads the step's lengths, which waits for it.
 """
 
 from __future__ import annotations
@@ -80,8 +80,9 @@ class PagedCache:
     """Key / value caches of ``layers`` layers for ``batch`` request places, in pages of ``page`` tokens.
 
     ``plan(new_lens)`` gives every place its new tokens' pages and slots; the packed token
-    rows of the step are the places' new tokens in order. The host keeps the lengths and
-    the free list, so a step reads nothing back."""
+    rows of the step are the places' new tokens in order. The host keeps the lengths, each
+    place's pages and the free list, so nothing is read back. With a window, pages that no later
+    token sees go back to the free list."""
 
     def __init__(self, ctx: L.Context, *, layers: int, batch: int, pages: int, page: int, heads: int, kv_heads: int, head_dim: int,
                  max_tokens: int, max_len: int, dtype: int = L.BF16, window: int = 0, sinks: int = 0, rope_base: float = 10000.0):
@@ -94,6 +95,7 @@ class PagedCache:
         self.v = [ctx.alloc(nbytes) for _ in range(layers)]
         self.lens = np.zeros(batch, np.int64)
         self.free = list(range(pages))
+        self.held = [{} for _ in range(batch)]   # place -> {index in its table row: page id}
         i32 = lambda n: ctx.alloc(4 * n)  # noqa: E731
         self.table = ctx.to_device(np.full((batch, self.stride), -1, np.int32))
         self.q_starts, self.kv_lens, self.slots, self.positions, self.status = (i32(n) for n in (batch + 1, batch, max_tokens, max_tokens, 2))
@@ -112,11 +114,13 @@ class PagedCache:
         """Pages, slots and positions for ``new_lens[b]`` new tokens of each place."""
         new = np.asarray(new_lens, np.int64)
         total = int(new.sum())
-        need = -(-(self.lens + new) // self.page) - -(-self.lens // self.page)
         if new.shape != (self.batch,) or (new < 0).any() or not 0 < total <= self.max_tokens:
             raise ValueError(f"new lengths for {self.batch} places, 1 to {self.max_tokens} tokens in all")
         if (self.lens + new > self.max_len).any():
             raise ValueError(f"a request would pass {self.max_len} tokens")
+        self._give_back()
+        held = -(-self.lens // self.page)
+        need = -(-(self.lens + new) // self.page) - held
         if need.sum() > len(self.free):
             raise L.MdlcError(L.ERR_NOMEM, f"{int(need.sum())} pages wanted, {len(self.free)} free")
         ctx, taken, max_q = self.ctx, int(need.sum()), int(new.max())
@@ -135,9 +139,20 @@ class PagedCache:
             ctx.upload(self._free, np.array(self.free[:taken], np.int32))
         desc = L.PageDesc(batch=self.batch, page=self.page, table_stride=self.stride, tokens=total, free_pages=taken)
         ctx.page_plan(desc, self._cached, self._new, self._free, 0, self.table, self.q_starts, self.kv_lens, self.slots, self.positions, self.status)
-        del self.free[:taken]
+        for b in range(self.batch):   # in the places' order, as the plan takes them
+            n = int(need[b])
+            self.held[b].update(zip(range(int(held[b]), int(held[b]) + n), self.free[:n]))
+            del self.free[:n]
         self.lens += new
         self.tokens, self.max_q = total, max_q
+
+    def _give_back(self) -> None:
+        """Pages behind the window: the next token stands at ``lens`` and sees keys from ``lens - window + 1`` on, and the sinks."""
+        if not self.window:
+            return
+        for b, held in enumerate(self.held):
+            for i in [i for i in held if (i + 1) * self.page <= self.lens[b] - self.window + 1 and i * self.page >= self.sinks]:
+                self.free.append(held.pop(i))
 
     def append(self, layer: int, qkv: int, q_out: int) -> None:
         """Rotate the queries of the packed [tokens][heads + 2 kv_heads][head_dim] projection into ``q_out`` and write its
@@ -159,10 +174,8 @@ class PagedCache:
         """End the request at ``place``: its pages go back to the free list."""
         if not 0 <= place < self.batch:
             raise ValueError(f"place {place} of {self.batch}")
-        held = -(-int(self.lens[place]) // self.page)
-        if held:
-            ids = self.ctx.download(self.table + 4 * place * self.stride, (held,), np.int32)
-            self.free.extend(int(i) for i in ids)
+        self.free.extend(self.held[place].values())
+        self.held[place] = {}
         self.lens[place] = 0
 
     def close(self) -> None:

@@ -34,7 +34,7 @@ class Books:
         self.uploads[p] = np.array(a)
 
     def download(self, p, shape, dtype):
-        raise AssertionError("a step reads nothing back")
+        raise AssertionError("nothing is read back")
 
     def sync(self):
         pass
@@ -87,3 +87,35 @@ def test_release_of_no_such_place(place):
     with pytest.raises(ValueError):
         c.release(place)
     assert list(c.lens) == [5, 6] and len(c.free) == 40 - 4
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (8, 0), (7, 0), (9, 5), (1, 1), (30, 4), (5, 100)])
+def test_pages_behind_the_window_are_given_back(rng, window, sinks):
+    """At every step a place holds exactly the pages of the keys that its next token can see (and with no window all), each page
+    belongs to one place or the free list, and the plan is given the pages that the host counts as taken."""
+    b, page = Books(), 4
+    c = cache(b, batch=3, pages=60, window=window, sinks=sinks)
+    for step in range(60):
+        new = rng.integers(0, 4, 3)
+        if step % 9 == 8:
+            place = int(rng.integers(0, 3))
+            c.release(place)
+            assert not c.held[place] and c.lens[place] == 0
+        new = np.minimum(new, c.max_len - c.lens)
+        if not new.sum():
+            continue
+        cached, before = c.lens.copy(), [dict(h) for h in c.held]
+        c.plan(new)
+        given = iter(b.plans[-1][2])
+        for i in range(3):
+            first = [j for j in range(-(-int(c.lens[i]) // page)) if j not in before[i]]
+            taken = [j for j in range(-(-int(cached[i]) // page), -(-int(c.lens[i]) // page))]
+            assert set(taken) <= set(first) and [c.held[i][j] for j in taken] == [next(given) for _ in taken]
+            # what this step's first token (position `cached`) sees is held, nothing else but the new tokens' pages
+            seen = {j for j in range(-(-int(cached[i]) // page)) if not window or (j + 1) * page > cached[i] - window + 1 or j * page < sinks}
+            assert set(c.held[i]) == seen | set(taken)
+        assert next(given, None) is None
+        ids = c.free + [p for h in c.held for p in h.values()]
+        assert sorted(ids) == list(range(60))
+    if window and window < 20 and sinks < 20:
+        assert max(len(h) for h in c.held) <= (window + sinks) // page + 4
