@@ -45,6 +45,13 @@ class Decoder:
         self.gate, self.upper = ctx.alloc(max_tokens * inner * esz), ctx.alloc(max_tokens * inner * esz)
         self.logits = ctx.alloc(max_tokens * vocab * 4)
 
+    def close(self):
+        self.cache.close()
+        for layer in (*self.qkv, *self.out, *self.up, *self.down, self.head):
+            layer.close()
+        for p in (*self.buf.values(), self.gate, self.upper, self.logits):
+            self.ctx.free(p)
+
     def _program(self, rows, width, inputs, code):
         p = L.EwProg(n=rows, hw=1, c=width, c_stride=width, dtype=self.dtype, n_inputs=inputs, n_outputs=1, n_instr=len(code))
         for i in range(inputs):
@@ -152,7 +159,7 @@ def run(steps=16, dtype="fp32", check=False, seed=0, **kw):
                     model.cache.release(i)           # answered: its pages serve the others
     ctx.sync()
     assert ctx.check_flag() == 0
-    model.cache.close()
+    model.close()
     ctx.close()
     return seqs, worst
 

@@ -75,6 +75,12 @@ class W4Linear:
                         y_type=dtype if out_dtype is None else out_dtype, x_stride=x_stride or self.k, y_stride=y_stride or self.n)
         self.ctx.gemv_w4(desc, x, self.codes, self.scales, self.zeros, self.bias, y)
 
+    def close(self) -> None:
+        """Frees the weights on the device; the layer cannot be called again."""
+        for p in filter(None, (self.codes, self.scales, self.zeros, self.bias)):
+            self.ctx.free(p)
+        self.codes = self.scales = self.zeros = self.bias = 0
+
 
 class PagedCache:
     """Key / value caches of ``layers`` layers for ``batch`` request places, in pages of ``page`` tokens.
@@ -179,6 +185,10 @@ class PagedCache:
         self.lens[place] = 0
 
     def close(self) -> None:
-        for p in (*self.k, *self.v, self.table, self.q_starts, self.kv_lens, self.slots, self.positions, self.status, self._cached, self._new,
-                  self._free, self.rope, self.workspace):
+        """Frees the caches and the plan's buffers; a second call does nothing."""
+        names = ("table", "q_starts", "kv_lens", "slots", "positions", "status", "_cached", "_new", "_free", "rope", "workspace")
+        for p in filter(None, (*self.k, *self.v, *(getattr(self, n) for n in names))):
             self.ctx.free(p)
+        self.k, self.v, self._room = [], [], 0
+        for n in names:
+            setattr(self, n, 0)

@@ -119,3 +119,19 @@ def test_pages_behind_the_window_are_given_back(rng, window, sinks):
         assert sorted(ids) == list(range(60))
     if window and window < 20 and sinks < 20:
         assert max(len(h) for h in c.held) <= (window + sinks) // page + 4
+
+
+def test_layers_and_caches_free_what_they_hold():
+    b = Books()
+    layers = [paged.W4Linear(b, np.ones((8, 64), np.float32), bias, group=32, zeros=z) for bias in (None, np.ones(8)) for z in (True, False)]
+    c = cache(b)
+    c.plan([3, 4])
+    for layer in layers:
+        layer(1, 1, 2, L.F32)
+        layer.close()
+        layer.close()
+        with pytest.raises(AssertionError):
+            layer(1, 1, 2, L.F32)
+    c.close()
+    c.close()
+    assert not b.live
