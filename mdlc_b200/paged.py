@@ -39,12 +39,15 @@ def quantize_w4(w: np.ndarray, group: int = 128, zeros: bool = True):
     if k % group:
         raise ValueError(f"k = {k} is not a multiple of the group {group}")
     g = np.asarray(w, np.float32).reshape(n, k // group, group)
+    if not np.isfinite(g).all():
+        raise ValueError("weights that are not finite")
     if zeros:
         lo, hi = np.minimum(g.min(-1), 0), np.maximum(g.max(-1), 0)
-        scale = (hi - lo) / 15
+        scale = hi / 15 - lo / 15
     else:
         scale = np.maximum(g.max(-1) / 7, -g.min(-1) / 8)
-    bits = _bf16_bits(np.where(scale > 0, scale, 1.0))
+    bits = _bf16_bits(scale)
+    bits = np.where(bits < 0x80, _bf16_bits(np.ones(1)), bits)   # all 0, or too small for a (normal) scale: every code stands for 0
     s = (bits.astype(np.uint32) << 16).view(np.float32)
     z = np.clip(np.rint(-lo / s), 0, 15) if zeros else np.full(s.shape, 8.0, np.float32)
     q = np.clip(np.rint(g / s[..., None]) + z[..., None], 0, 15).astype(np.uint8).reshape(n, k)

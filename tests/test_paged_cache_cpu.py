@@ -135,3 +135,24 @@ def test_layers_and_caches_free_what_they_hold():
     c.close()
     c.close()
     assert not b.live
+
+
+@pytest.mark.parametrize("zeros", [True, False])
+def test_quantize_w4_of_tiny_and_large_weights(rng, zeros):
+    """Weights too small for a bf16 scale become 0, the largest ones stay finite, others beside them keep their own scale."""
+    with np.errstate(all="raise", under="ignore"):
+        for size in (1e-41, 1e-39, 1e-30, 3e38):
+            w = rng.uniform(-1, 1, (3, 96)).astype(np.float32)
+            w[1, 32:64] = rng.uniform(-1, 1, 32) * size
+            codes, bits, z = paged.quantize_w4(w, 32, zeros)
+            scale = (bits.astype(np.uint32) << 16).view(np.float32)
+            assert np.isfinite(scale).all() and (scale > 0).all()
+            got = paged.dequantize_w4(codes, bits, z).reshape(3, 3, 32)
+            err = abs(got.astype(np.float64) - w.reshape(3, 3, 32)).max(-1)
+            # a step or, in the group that has no scale, the weights themselves
+            assert (err <= np.where(scale == 1, size, 1.01 * scale)).all()
+    for bad in (np.nan, np.inf, -np.inf):
+        w = np.zeros((2, 64), np.float32)
+        w[1, 40] = bad
+        with pytest.raises(ValueError):
+            paged.quantize_w4(w, 32, zeros)
