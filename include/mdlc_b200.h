@@ -494,12 +494,12 @@ int mdlc_paged_attn(mdlc_ctx* ctx, const mdlc_attn_desc* desc, const void* q, co
  *   y[i][o] = bias[o] + sum_c x[i][c] (code[o][c] - zero[o][c / group]) scale[o][c / group]
  * codes: [n][k / 2] bytes, column c in the low (c even) or high (c odd) nibble of
  * byte c / 2; scales: [n][k / group] bf16; zeros: [n][k / group] uint8 0..15, null:
- * 8; bias: [n] fp32 or null. x is taken to 23 bits of the largest |x| of each row's 128
- * columns (what an fp32 product with that one would round), products and a group's sums
- * are exact, groups are added in fp32; a non-finite x gives a non-finite y. codes 16-byte
+ * 8; bias: [n] fp32 or null. Products are exact for both types of x (below 2^-110 an
+ * fp32 x loses its last bits), sums are fp32: a column of x that is far above the others
+ * takes nothing from them. Non-finite x as in IEEE arithmetic, scales finite. codes 16-byte
  * aligned; x 16-byte aligned with x_stride a multiple of 8. Uses the context's split-K workspace. */
 typedef struct {
-  int32_t m;     /* rows, at most 65535; made for 1 .. 16, more re-read the weights */
+  int32_t m;     /* rows, at most 65535; 48 bf16 or 16 fp32 rows share a read of the weights */
   int32_t n;     /* output columns */
   int32_t k;     /* a multiple of group */
   int32_t group; /* 32, 64 or 128 */

@@ -2,20 +2,16 @@
 //
 // Memory-bound: half a byte of weight per 2 m operations. At the copy bandwidth an SM receives 48
 // weights a clock, so what decides, besides bytes in flight, is how many instructions a weight
-// costs. The products therefore run on the int8 tensor pipe (mma.sync m16n8k32, exact int32 sums), where
-// eight codes need three integer operations and one product:
-//   * the weights are the 16-row operand. Code - 8 of the high nibbles of a word is
-//     (w & 0xf0f0f0f0) ^ 0x80808080, read as four signed bytes 16 (code - 8); the low nibbles likewise
-//     after one shift. (As bf16 operands they took 11 operations, two of them per pair of
-//     codes, and the kernel was bound by the integer pipe: 79 us at one row of 65536 x 8192 where this
-//     one takes 56 us, 4.9 TB/s.)
-//   * x is written once as fixed-point numbers of 23 bits, a power of two per row and 128 columns
-//     (the largest magnitude just below 2^22), cut into three balanced signed base-256 digits, each a
-//     column of the 8-column operand. The error is at most 2^-23 of the largest |x| of those columns: what an fp32 product
-//     with that element would round.
-//   * a group's int32 sums (below 2^21) start from the bits of 1.5 x 2^23, so they are fp32 numbers as they
-//     stand; they are scaled and added to the row's fp32 sum once per group. A zero point z other
-//     than 8 adds (8 - z) times the digits' sum.
+// costs. The products run on the bf16 tensor pipe (mma.sync m16n8k16, fp32 sums), every one of them exact:
+//   * the weights are the 16-row operand. A code c or-ed into the low mantissa bits of 2^-5 is 2^-5 + c 2^-12, and less
+//     2^-5 + z 2^-12 (z the zero point) it is (c - z) 2^-12 exactly: eleven operations for eight codes. The factor, which the
+//     end takes off again, keeps a group's sums below the largest |x| of it.
+//   * x is the 8-column operand: a bf16 row is one column as it is, an fp32 row three, whose sum it is exactly (8 bits each, cut
+//     off in turn; below 2^-110 the last bits go). No scale is shared between columns of x, so a large one that meets weights of
+//     zero takes nothing from its neighbours. (Fixed-point digits with a shared scale on the int8 pipe cost three operations for
+//     eight codes - one row of 65536 x 8192 55 us, here 67 us, 4.1 TB/s - but an error that followed the largest |x| of 128
+//     columns, and three columns for a bf16 row too: 16 rows of 14336 x 4096 51 us, here 33 us.)
+//   * a group is summed from zero in the tensor core, scaled and added to the row's fp32 sum.
 // The order of the columns inside a product is free as long as both operands agree, so a thread keeps
 // the 32 consecutive codes of its 16-byte load. For groups under 128 columns the four threads of a row hold different
 // groups; a 4 x 4 exchange of words inside the quad then puts 32 consecutive columns into each product.
@@ -32,8 +28,9 @@ namespace {
 
 constexpr int kW4Warps = 8;
 constexpr int kW4Depth = 4;        // 128-column steps of weights on their way per warp
-constexpr int kW4OwnX = 41 * 1024;  // x that a block turns into digits itself (one row) at most
-constexpr uint32_t kMagic = 0x4b400000u;  // 1.5 x 2^23: adding an integer below 2^22 to the bits adds it to the number
+constexpr int kW4OwnX = 41 * 1024;  // x that a block splits itself (one row) at most
+constexpr uint32_t kCode0 = 0x3d003d00u;  // two bf16 numbers 2^-5; one more in the last place is 2^-12
+constexpr float kCodeUnit = 4096.0f;      // 2^12
 
 struct W4Args {
   mdlc_w4_desc d;
@@ -44,10 +41,11 @@ struct W4Args {
   const float* bias;
   void* y;
   int rows_per_chunk;   // x rows of one grid.y chunk
+  int parts;            // columns of an x row: 1 (bf16) or 3 (fp32)
   int pitch;            // columns kept per 8 of k
-  int step_bytes;       // x of one step, see w4_step_bytes
+  int step_bytes;       // x of one step: 16 units of 8 columns x pitch x 16 bytes
   int span, buffers;    // steps in shared memory at a time, and their buffers
-  const uint8_t* ready; // x as digits, [chunk][step], or null: the block makes them itself
+  const uint8_t* ready; // x in parts, [chunk][step], or null: the block makes them itself
   bool ready_wanted;
   int* err;
 };
@@ -57,16 +55,17 @@ MDLC_DEV void cp_async_16_all(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-MDLC_DEV void mma_s8(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+MDLC_DEV void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// the high nibble of each byte as a signed byte 16 (code - 8)
-MDLC_DEV uint32_t high_codes(uint32_t w) {
+// the codes in bits 0-3 and 16-19 as two bf16 numbers (code - z) 2^-12; zero: kCode0 with z in both halves
+MDLC_DEV uint32_t code_pair(uint32_t w, uint32_t zero) {
   uint32_t v;
-  asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(v) : "r"(w), "r"(0xf0f0f0f0u), "r"(0x80808080u));  // (a & b) ^ c
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(w), "r"(0x000f000fu), "r"(kCode0));  // (a & b) | c
+  asm("sub.rn.bf16x2 %0, %0, %1;" : "+r"(v) : "r"(zero));
   return v;
 }
 
@@ -84,98 +83,86 @@ MDLC_DEV void quad_transpose(uint32_t (&w)[4], int t) {
   }
 }
 
-// x as digits, one 128-column step of k after the other, each: 16 units of 8 columns x pitch columns x 8 bytes (the digits of
-// columns 0, 2, 4, 6 and 1, 3, 5, 7; units and columns permuted so that the four units a warp reads at once,
-// 4 apart or adjacent, lie in different banks); the columns' weights / 256 (fp32); per group of the weights the digits' sums (fp32)
+// x in parts, one 128-column step of k after the other, each: 16 units of 8 columns x pitch columns x 16 bytes (bf16, columns
+// 0 4 1 5 2 6 3 7 of the unit, as the codes of a word come). Units and columns are permuted so that the four units a warp reads
+// at once, 4 apart or adjacent, lie in different banks for each pair of columns.
 MDLC_DEV int x_place(int unit, int col, int pitch) {
-  const int v = unit ^ ((unit >> 2) & 3);
-  return v * pitch + (pitch == 4 ? col : col ^ ((v & 2) << 1));
+  const int turn = (unit ^ (unit >> 2)) & 3;
+  if (pitch == 1) return (unit & ~3) | turn;
+  if (pitch == 4) return ((unit & ~3) | turn) * 4 + (col ^ (turn & 2));
+  return unit * pitch + (col ^ (2 * turn));
 }
-__host__ __device__ inline int w4_step_bytes(int pitch, int group) { return pitch * (128 + 4 + 128 / group * 4); }
 
-// Eight columns of an x row as digits, by one lane; the 16 lanes of a step (neighbours) share an exponent. u: unit; dst: the
-// step that holds it. Every lane of the warp calls this; `ok`: the unit is one of a step's (past k: zeros).
-MDLC_DEV void x_digits(const float (&f)[8], int u, int col0, int group, int pitch, uint8_t* dst, bool ok) {
-  const int per = group / 8;
-  uint32_t top = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  // |x| < 2^(ex - 126); below 2^-96 the digits get shorter
-  const bool finite = top < 0x7f800000u;
-  const int ex = max((int)(top >> 23), 30);
-  const float up = __uint_as_float((uint32_t)(275 - ex) << 23);  // 2^(148 - ex)
-  uint32_t y[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    y[e] = (__float_as_uint(fminf(fmaxf(f[e] * up, -4194303.0f), 4194303.0f) + __uint_as_float(kMagic)) - kMagic + 0x808080u) ^ 0x808080u;
-  // 1/16 for the weights' factor, and 1/16 that the end restores: no digit's sum overflows where their sum does not
-  float down = __uint_as_float((uint32_t)(ex - 29) << 23);  // 2^(ex - 156)
-  if (!finite) {
-    // infinities become the digit +-1 (the finite columns beside them 0) of an infinite weight, NaN a NaN weight
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = (__float_as_uint(f[e]) & 0x7fffffffu) == 0x7f800000u ? (f[e] > 0.0f ? 1u : 0xffu) : 0u;
-    down = __uint_as_float(top);
+// Unit u of an x row in its parts, written to the step that holds it (past k: zeros). col0: the row's first column
+template <bool BF16>
+MDLC_DEV void x_unit(const W4Args& a, const uint4 (&raw)[2], int u, int col0, uint8_t* dst) {
+  uint4* units = reinterpret_cast<uint4*>(dst);
+  if (BF16) {
+    const uint4 p = raw[0];
+    units[x_place(u & 15, col0, a.pitch)] = make_uint4(__byte_perm(p.x, p.z, 0x5410), __byte_perm(p.x, p.z, 0x7632), __byte_perm(p.y, p.w, 0x5410),
+                                                       __byte_perm(p.y, p.w, 0x7632));
+    return;
   }
-  uint2* units = reinterpret_cast<uint2*>(dst);
-  float* xf = reinterpret_cast<float*>(dst + 128 * pitch);
+  const uint32_t f[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+  uint32_t part[3][8];  // bf16 in the upper half
 #pragma unroll
-  for (int p = 0; p < 3; ++p) {
-    const uint32_t two = p | ((4 + p) << 4);
-    uint2 b;
-    b.x = __byte_perm(__byte_perm(y[0], y[2], two), __byte_perm(y[4], y[6], two), 0x5410);
-    b.y = __byte_perm(__byte_perm(y[1], y[3], two), __byte_perm(y[5], y[7], two), 0x5410);
-    if (ok) units[x_place(u & 15, col0 + p, pitch)] = b;
-    int sum = __dp4a((int)b.x, 0x01010101, __dp4a((int)b.y, 0x01010101, 0));
-    for (int o = 1; o < per; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (ok && (u & 15) == 0) xf[col0 + p] = p == 0 ? down : (finite ? down * (p == 1 ? 256.0f : 65536.0f) : 0.0f);
-    if (ok && (u & (per - 1)) == 0) xf[(1 + (u & 15) / per) * pitch + col0 + p] = (float)sum;
+  for (int e = 0; e < 8; ++e) {
+    const uint32_t top = f[e] & 0x7fffffffu;
+    part[0][e] = top > 0x7f800000u ? 0x7fc00000u : f[e] & 0xffff0000u;  // (a NaN's upper bits alone may be an infinity's)
+    const float rest = top < 0x7f800000u ? __uint_as_float(f[e]) - __uint_as_float(part[0][e]) : 0.0f;
+    part[1][e] = __float_as_uint(rest) & 0xffff0000u;
+    part[2][e] = __float_as_uint(rest - __uint_as_float(part[1][e]));
   }
+#pragma unroll
+  for (int p = 0; p < 3; ++p)
+    units[x_place(u & 15, col0 + p, a.pitch)] = make_uint4(__byte_perm(part[p][0], part[p][4], 0x7632), __byte_perm(part[p][1], part[p][5], 0x7632),
+                                                           __byte_perm(part[p][2], part[p][6], 0x7632), __byte_perm(part[p][3], part[p][7], 0x7632));
 }
-MDLC_DEV void x_load(const W4Args& a, int row, int u, bool ok, float (&f)[8]) {
-  uint4 p = make_uint4(0, 0, 0, 0), v = p;
-  if (ok) {
-    const long long at = (long long)row * a.d.x_stride + u * 8;
-    if (a.d.x_type == MDLC_BF16) {
-      p = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.x) + at));
-    } else {
-      p = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(a.x) + at));
-      v = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(a.x) + at) + 1);
-    }
-  }
-  if (a.d.x_type == MDLC_BF16) {
-    f[0] = bf16_lo(p.x); f[1] = bf16_hi(p.x); f[2] = bf16_lo(p.y); f[3] = bf16_hi(p.y);
-    f[4] = bf16_lo(p.z); f[5] = bf16_hi(p.z); f[6] = bf16_lo(p.w); f[7] = bf16_hi(p.w);
+template <bool BF16>
+MDLC_DEV void x_load(const W4Args& a, int row, int u, bool ok, uint4 (&raw)[2]) {
+  raw[0] = raw[1] = make_uint4(0, 0, 0, 0);
+  if (!ok) return;
+  const long long at = (long long)row * a.d.x_stride + u * 8;
+  if (BF16) {
+    raw[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.x) + at));
   } else {
-    f[0] = __uint_as_float(p.x); f[1] = __uint_as_float(p.y); f[2] = __uint_as_float(p.z); f[3] = __uint_as_float(p.w);
-    f[4] = __uint_as_float(v.x); f[5] = __uint_as_float(v.y); f[6] = __uint_as_float(v.z); f[7] = __uint_as_float(v.w);
+    raw[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(a.x) + at));
+    raw[1] = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(a.x) + at) + 1);
   }
 }
 
-// x as digits in global memory, for the blocks of gemv_w4_kernel to copy: a warp per row and 256 columns
-__global__ void __launch_bounds__(128) w4_digits_kernel(const W4Args a, uint8_t* ready) {
+// x in parts in global memory, for the blocks of gemv_w4_kernel to copy: a thread per row and unit
+template <bool BF16>
+__global__ void __launch_bounds__(128) w4_parts_kernel(const W4Args a, uint8_t* ready) {
   pdl_wait();
   pdl_trigger();
-  const int units = a.d.k / 8, lane = threadIdx.x & 31, steps = (a.d.k + 127) / 128;
-  const int u = (blockIdx.x * 4 + (threadIdx.x >> 5)) * 32 + lane, row = blockIdx.y;
-  float f[8];
-  x_load(a, row, u, u < units, f);
+  const int steps = (a.d.k + 127) / 128, u = blockIdx.x * 128 + threadIdx.x, row = blockIdx.y;
+  if (u >= 16 * steps) return;
+  uint4 raw[2];
+  x_load<BF16>(a, row, u, u < a.d.k / 8, raw);
   const int chunk = row / a.rows_per_chunk;
-  uint8_t* dst = ready + ((long long)chunk * steps + min(u / 16, steps - 1)) * a.step_bytes;
-  x_digits(f, u, 3 * (row - chunk * a.rows_per_chunk), a.d.group, a.pitch, dst, u < 16 * steps);
+  x_unit<BF16>(a, raw, u, a.parts * (row - chunk * a.rows_per_chunk), ready + ((long long)chunk * steps + u / 16) * a.step_bytes);
+}
+
+// all of one row into shared memory, by the whole block
+template <bool BF16>
+MDLC_DEV void x_own(const W4Args& a, int row, int steps, uint8_t* xs) {
+  const int units = a.d.k / 8;
+  constexpr int N = kW4Warps * 32;
+  for (int u0 = threadIdx.x; u0 < 16 * steps; u0 += 2 * N) {  // two loads at a time
+    const int u1 = u0 + N;
+    uint4 r0[2], r1[2];
+    x_load<BF16>(a, row, u0, u0 < units, r0);
+    x_load<BF16>(a, row, u1, u1 < units, r1);
+    x_unit<BF16>(a, r0, u0, 0, xs + u0 / 16 * a.step_bytes);
+    if (u1 < 16 * steps) x_unit<BF16>(a, r1, u1, 0, xs + u1 / 16 * a.step_bytes);
+  }
 }
 
 // a run of bytes (16-byte aligned, a multiple of 16) into shared memory, completing on an mbarrier
 MDLC_DEV void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
                : "memory");
-}
-
-MDLC_DEV float2 add2(const float2 a, const float2 b) {
-  unsigned long long r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f2_bits(a)), "l"(f2_bits(b)));
-  return f2_from(r);
 }
 
 // NT: 8-column tiles; R: 16-row tiles; GROUP: columns of a group; ZEROS: zero points given
@@ -233,7 +220,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
       enter();
     }
   };
-  // scales and zero points of a step's groups (past k: the last group's, for columns whose digits are 0)
+  // scales and zero points of a step's groups (past k: 0, for columns whose x is 0)
   constexpr int SETS = 128 / GROUP;
   uint32_t sc[SETS][R][2] = {}, sc_next[SETS][R][2] = {}, zr[SETS][R][2] = {}, zr_next[SETS][R][2] = {};
   int s_tile = blockIdx.x, s_step = warp;
@@ -253,13 +240,13 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
     if (s_tile < tiles && s_step < steps) {
 #pragma unroll
       for (int i = 0; i < SETS; ++i) {
-        const uint32_t grp = G128 ? s_step : min(s_step * SETS + i, groups - 1);
+        const int grp = s_step * SETS + i;
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            sc_next[i][r][h] = __ldg(sp[r][h] + grp);
-            if (ZEROS) zr_next[i][r][h] = __ldg(zp[r][h] + grp);
+            sc_next[i][r][h] = G128 || grp < groups ? __ldg(sp[r][h] + grp) : 0;
+            if (ZEROS) zr_next[i][r][h] = G128 || grp < groups ? __ldg(zp[r][h] + grp) : 0;
           }
       }
     }
@@ -276,11 +263,11 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
   for (int i = 0; i < kW4Depth - 1; ++i) load(ring + i * kSlot);
   enter_scales();
   load_scales();
-  // where this thread's four units of a step lie (column tile j: 64 bytes on)
+  // where this thread's four units of a step lie (column tile j: 128 bytes on)
   uint32_t x_off[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x_off[i] = 8 * x_place(G128 ? 4 * t + i : 4 * i + t, pitch == 4 ? g & 3 : g, pitch);
-  const uint32_t xs_addr = smem_u32(xs), f_off = 128 * pitch + 4 * (pitch == 4 ? (2 * t) & 3 : 2 * t);
+  for (int i = 0; i < 4; ++i) x_off[i] = 16 * x_place(G128 ? 4 * t + i : 4 * i + t, pitch == 4 ? g & 3 : g, pitch);
+  const uint32_t xs_addr = smem_u32(xs);
 
   // x: one buffer for all of it, or two that the spans of every tile take in turn, the next one on its way
   const int spans = (steps + a.span - 1) / a.span;
@@ -298,16 +285,10 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
       fence_mbar_init();
       fetch_x(0);
     }
+  } else if (d.x_type == MDLC_BF16) {
+    x_own<true>(a, m0, steps, xs);
   } else {
-    const int units = d.k / 8;
-    for (int u0 = warp * 32; u0 < 16 * steps; u0 += 2 * kW4Warps * 32) {  // two loads at a time
-      const int u1 = u0 + kW4Warps * 32 + lane, ua = u0 + lane;
-      float fa[8], fb[8];
-      x_load(a, m0, ua, ua < units, fa);
-      x_load(a, m0, u1, u1 < units, fb);
-      x_digits(fa, ua, 0, GROUP, pitch, xs + min(ua / 16, steps - 1) * a.step_bytes, ua < 16 * steps);
-      x_digits(fb, u1, 0, GROUP, pitch, xs + min(u1 / 16, steps - 1) * a.step_bytes, u1 < 16 * steps);
-    }
+    x_own<false>(a, m0, steps, xs);
   }
   __syncthreads();
 
@@ -326,7 +307,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
       }
       const uint8_t* buf = xs + (spans > 1 ? (q - 1) & 1 : 0) * x_bytes;
       const int s1 = min(steps, s0 + a.span);
-      for (int s = s0 + warp; s < s1; s += kW4Warps) {
+      for (int s = s0 + ((warp - s0) & (kW4Warps - 1)); s < s1; s += kW4Warps) {  // step s is warp s % 8's
 #pragma unroll
         for (int i = 0; i < SETS; ++i)
 #pragma unroll
@@ -350,63 +331,53 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
           }
         slot = (slot + 1) % kW4Depth;
         const uint8_t* x_at = buf + (s - s0) * a.step_bytes;
-        uint32_t acc[R][NT][4];
-        float2 part[R][NT][2] = {};  // the step's sums of scaled groups
+        float acc[R][NT][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           // word i holds columns 32 t + 8 i of this step (G128) or, after the exchange, 32 i + 8 t
-          const bool first = G128 ? i == 0 : 32 * i % GROUP == 0;
+          const bool first = G128 ? i == 0 : 32 * i % GROUP == 0, last = G128 ? i == 3 : 32 * (i + 1) % GROUP == 0;
+          const int set = G128 ? 0 : 32 * i / GROUP;
           if (first) {
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
               for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[r][j][e] = kMagic;
+                for (int e = 0; e < 4; ++e) acc[r][j][e] = 0.0f;
           }
-          // columns without an x row read what lies there (a single row's are read twice): their sums are not used
-          uint2 b[NT];
+          // columns without an x row read what lies there (a single row's are read several times): their sums are not used
+          uint4 b[NT];
 #pragma unroll
-          for (int j = 0; j < NT; ++j) b[j] = *reinterpret_cast<const uint2*>(x_at + x_off[i] + 64 * j);
+          for (int j = 0; j < NT; ++j) b[j] = *reinterpret_cast<const uint4*>(x_at + x_off[i] + 128 * j);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
-            const uint32_t a0 = high_codes(w[r][0][i] << 4), a1 = high_codes(w[r][1][i] << 4);
-            const uint32_t a2 = high_codes(w[r][0][i]), a3 = high_codes(w[r][1][i]);
+            uint32_t c[4][2];  // columns n and n + 4 of the word, rows g and g + 8
 #pragma unroll
-            for (int j = 0; j < NT; ++j) mma_s8(acc[r][j], a0, a1, a2, a3, b[j].x, b[j].y);
-          }
-          const bool last = G128 ? i == 3 : 32 * (i + 1) % GROUP == 0;
-          if (last) {
-            const int set = G128 ? 0 : 32 * i / GROUP;
-            const uint8_t* dp = x_at + f_off + (1 + set) * pitch * 4;
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t zero = ZEROS ? kCode0 + (zr[set][r][h] & 15u) * 0x00010001u : kCode0 + 0x00080008u;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              float2 dx = splat2(0.0f);
-              if (ZEROS) dx = *reinterpret_cast<const float2*>(dp + 32 * j);
-#pragma unroll
-              for (int r = 0; r < R; ++r)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  float2 f = splat2(-12582912.0f);
-                  if (ZEROS) f = fma2(splat2(__uint_as_float(kMagic + 128u - 16u * (zr[set][r][h] & 15u)) - 12582912.0f), dx, f);
-                  f = add2(make_float2(__uint_as_float(acc[r][j][2 * h]), __uint_as_float(acc[r][j][2 * h + 1])), f);
-                  part[r][j][h] = fma2(splat2(__uint_as_float(sc[set][r][h] << 16)), f, part[r][j][h]);
-                }
+              for (int n = 0; n < 4; ++n) c[n][h] = code_pair(w[r][h][i] >> (4 * n), zero);
             }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) mma_bf16(acc[r][j], c[0][0], c[0][1], c[1][0], c[1][1], b[j].x, b[j].y);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) mma_bf16(acc[r][j], c[2][0], c[2][1], c[3][0], c[3][1], b[j].z, b[j].w);
           }
-        }
+          if (last) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const float2 fx = *reinterpret_cast<const float2*>(x_at + f_off + 32 * j);
+            for (int r = 0; r < R; ++r)
 #pragma unroll
-          for (int r = 0; r < R; ++r)
+              for (int h = 0; h < 2; ++h) {
+                const float2 scale = splat2(__uint_as_float(sc[set][r][h] << 16));
 #pragma unroll
-            for (int h = 0; h < 2; ++h) out[r][j][h] = fma2(fx, part[r][j][h], out[r][j][h]);
+                for (int j = 0; j < NT; ++j) out[r][j][h] = fma2(scale, make_float2(acc[r][j][2 * h], acc[r][j][2 * h + 1]), out[r][j][h]);
+              }
+          }
         }
       }
     }
 
-    // sums of the digits and of the warps: eight neighbouring threads per output, a warp's sums each, added in a fixed tree
+    // sums of the parts and of the warps: eight neighbouring threads per output, a warp's sums each, added in a fixed tree
     constexpr int RP = 8 * NT + 2, ROWS = 16 * R;
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -417,12 +388,13 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
     __syncthreads();
     for (int i = threadIdx.x; i < ROWS * mc * kW4Warps; i += kW4Warps * 32) {
       const int w = i % kW4Warps, o = i / kW4Warps % ROWS, xr = i / (kW4Warps * ROWS), n = tile * ROWS + o;
-      const float* p = red + (w * ROWS + o) * RP + xr * 3;
-      float v = (p[0] + p[1]) + p[2];  // the small digits first
+      const float* p = red + (w * ROWS + o) * RP + xr * a.parts;
+      // the small parts first; they do not change an infinity (an infinite scale may have made them 0 x inf)
+      float v = a.parts == 1 || isinf(p[0]) ? p[0] : (p[2] + p[1]) + p[0];
 #pragma unroll
       for (int x = 1; x < kW4Warps; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
       if (w == 0 && n < d.n) {
-        v *= 16.0f;
+        v *= kCodeUnit;
         if (a.bias) v += __ldg(a.bias + n);
         const long long at = (long long)(m0 + xr) * d.y_stride + n;
         if (d.y_type == MDLC_BF16) static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
@@ -452,7 +424,8 @@ W4Plan w4_plan(const W4Args& a, int num_sms) {
       q.span = steps;
       q.buffers = 1;
     } else {
-      q.span = a.ready_wanted ? max(0, room) / 2 / a.step_bytes / kW4Warps * kW4Warps : 0;
+      q.span = a.ready_wanted ? max(0, room) / 2 / a.step_bytes : 0;
+      if (q.span > kW4Warps) q.span -= q.span % kW4Warps;  // whole rounds of the warps, where there is room for one
       q.buffers = 2;
     }
     q.smem = rest + q.buffers * q.span * a.step_bytes;
@@ -484,18 +457,19 @@ cudaError_t launch_w4(mdlc_ctx* ctx, W4Args& a, const W4Plan& p) {
 
 template <int NT>
 cudaError_t launch_w4_cols(mdlc_ctx* ctx, W4Args& a) {
-  a.rows_per_chunk = 8 * NT / 3;
-  a.pitch = a.d.m == 1 ? 4 : 8 * NT;
-  a.step_bytes = w4_step_bytes(a.pitch, a.d.group);
+  a.parts = a.d.x_type == MDLC_BF16 ? 1 : 3;
+  a.rows_per_chunk = 8 * NT / a.parts;
+  a.pitch = a.d.m == 1 ? (a.parts == 1 ? 1 : 4) : 8 * NT;
+  a.step_bytes = 256 * a.pitch;
   const long long steps = ((long long)a.d.k + 127) / 128;
   const bool ready = a.ready_wanted = a.d.m > 1 || steps * a.step_bytes > kW4OwnX;
-  // several rows: one kernel makes the digits for all blocks, as many chunks of rows at a time as the context's workspace holds
+  // several rows: one kernel splits them for all blocks, as many chunks of rows at a time as the context's workspace holds
   const long long fit = (long long)kSplitWsBytes / (steps * a.step_bytes);
   if (ready && fit == 0) return cudaErrorNotSupported;
   const int m = a.d.m, batch = ready ? (int)min((long long)m, fit * a.rows_per_chunk) : m;
   const W4Plan one = w4_plan<NT, 1>(a, ctx->num_sms), two = w4_plan<NT, 2>(a, ctx->num_sms);
   // Two row tiles share a read of x: a round of them takes less than two of single ones. The fewer and fuller
-  // rounds win (65536 rows: 7 rounds of two tiles 56 us, 14 of one 66 us; 4096 rows: one round either way).
+  // rounds win (65536 rows: 7 rounds of two tiles 67 us; 4096 rows: one round either way).
   const bool pair = two.span && (!one.span || 3 * two.rounds() < 2 * one.rounds());
   for (int m0 = 0; m0 < m; m0 += batch) {
     W4Args b = a;
@@ -503,11 +477,13 @@ cudaError_t launch_w4_cols(mdlc_ctx* ctx, W4Args& a) {
     b.x = static_cast<const char*>(a.x) + (long long)m0 * a.d.x_stride * (a.d.x_type == MDLC_BF16 ? 2 : 4);
     b.y = static_cast<char*>(a.y) + (long long)m0 * a.d.y_stride * (a.d.y_type == MDLC_BF16 ? 2 : 4);
     if (ready) {
-      uint8_t* digits = reinterpret_cast<uint8_t*>(ctx->d_split_ws);
+      uint8_t* parts = reinterpret_cast<uint8_t*>(ctx->d_split_ws);
       mdlc_note_launch(ctx);
-      const cudaError_t e = launch_pdl(w4_digits_kernel, dim3((unsigned)((steps * 16 + 127) / 128), b.d.m), dim3(128), 0, ctx->stream, b, digits);
+      const dim3 grid((unsigned)((steps * 16 + 127) / 128), b.d.m);
+      const cudaError_t e = a.parts == 1 ? launch_pdl(w4_parts_kernel<true>, grid, dim3(128), 0, ctx->stream, b, parts)
+                                         : launch_pdl(w4_parts_kernel<false>, grid, dim3(128), 0, ctx->stream, b, parts);
       if (e != cudaSuccess) return e;
-      b.ready = digits;
+      b.ready = parts;
     }
     mdlc_note_launch(ctx);
     const cudaError_t e = pair ? launch_w4<NT, 2>(ctx, b, two) : launch_w4<NT, 1>(ctx, b, one);
@@ -517,9 +493,12 @@ cudaError_t launch_w4_cols(mdlc_ctx* ctx, W4Args& a) {
 }
 
 cudaError_t launch_w4_rows(mdlc_ctx* ctx, W4Args& a) {
-  // Three columns per row, up to 16 rows in six column tiles at once. (Fewer tiles at once would let all of x stay in shared memory, but
-  // read the weights again: 16 rows of 14336 x 4096 in six tiles 40 us, in three, twice, 53 us.)
-  const int need = (int)min(6ll, (3ll * a.d.m + 7) / 8), nt = need == 5 ? 6 : need;
+  // Up to six column tiles at once: 48 bf16 rows, 16 fp32 rows. Fewer where the parts of one chunk would not fit the workspace.
+  const long long steps = ((long long)a.d.k + 127) / 128;
+  const int parts = a.d.x_type == MDLC_BF16 ? 1 : 3;
+  int nt = (int)min(6ll, ((long long)parts * a.d.m + 7) / 8);
+  nt = (int)min((long long)nt, max(1ll, (long long)kSplitWsBytes / (steps * 256 * 8)));
+  if (nt == 5) nt = 6 * steps * 256 * 8 <= (long long)kSplitWsBytes ? 6 : 4;
   switch (nt) {
     case 1: return launch_w4_cols<1>(ctx, a);
     case 2: return launch_w4_cols<2>(ctx, a);
@@ -549,7 +528,7 @@ extern "C" int mdlc_gemv_w4(mdlc_ctx* ctx, const mdlc_w4_desc* d, const void* x,
     return mdlc_set_error(ctx, MDLC_ERR_INVALID, "gemv_w4: misaligned pointer");
   if (d->m > 65535) return mdlc_set_error(ctx, MDLC_ERR_UNSUPPORTED, "gemv_w4: %d rows (at most 65535)", d->m);
   cudaSetDevice(ctx->device);
-  W4Args a = {*d, x, codes, static_cast<const uint16_t*>(scales), zeros, bias, y, 0, 0, 0, 0, 0, nullptr, false, ctx->d_err};
+  W4Args a = {*d, x, codes, static_cast<const uint16_t*>(scales), zeros, bias, y, 0, 0, 0, 0, 0, 0, nullptr, false, ctx->d_err};
   const cudaError_t e = launch_w4_rows(ctx, a);
   if (e == cudaErrorNotSupported) return mdlc_set_error(ctx, MDLC_ERR_UNSUPPORTED, "gemv_w4: k = %d does not fit the workspace", d->k);
   return mdlc_cuda_status(ctx, e, "gemv_w4 launch");
