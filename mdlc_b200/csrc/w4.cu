@@ -28,7 +28,9 @@ namespace {
 
 constexpr int kW4Warps = 8;
 constexpr int kW4Depth = 4;        // 128-column steps of weights on their way per warp
-constexpr int kW4OwnX = 41 * 1024;  // x that a block splits itself (one row) at most
+// A single row up to this long is split by every block itself (fp32, 8192 columns, 28672 outputs: 50.8 us, 56.2 with a kernel in front;
+// bf16, 28672 columns, 8192 outputs: 42.7 and 39.5)
+constexpr int kW4OwnColumns = 12288;
 constexpr uint32_t kCode0 = 0x3d003d00u;  // two bf16 numbers 2^-5; one more in the last place is 2^-12
 constexpr float kCodeUnit = 4096.0f;      // 2^12
 
@@ -462,7 +464,7 @@ cudaError_t launch_w4_cols(mdlc_ctx* ctx, W4Args& a) {
   a.pitch = a.d.m == 1 ? (a.parts == 1 ? 1 : 4) : 8 * NT;
   a.step_bytes = 256 * a.pitch;
   const long long steps = ((long long)a.d.k + 127) / 128;
-  const bool ready = a.ready_wanted = a.d.m > 1 || steps * a.step_bytes > kW4OwnX;
+  const bool ready = a.ready_wanted = a.d.m > 1 || a.d.k > kW4OwnColumns;
   // several rows: one kernel splits them for all blocks, as many chunks of rows at a time as the context's workspace holds
   const long long fit = (long long)kSplitWsBytes / (steps * a.step_bytes);
   if (ready && fit == 0) return cudaErrorNotSupported;

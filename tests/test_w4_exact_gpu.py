@@ -59,7 +59,7 @@ def random_case(rng, m, n, k, group, zeros, bias, xt):
     ("bf16", 1, 9472, 256, 128, 0, 0), ("bf16", 1, 9600, 544, 32, 1, 1), ("f32", 1, 18944, 384, 64, 1, 0), ("bf16", 8, 20011, 256, 64, 0, 1),
     ("bf16", 16, 20000, 640, 128, 1, 0), ("f32", 16, 9500, 256, 32, 0, 0), ("f32", 3, 19000, 288, 32, 1, 0),
     # a single row that is too long for the blocks to split themselves
-    ("bf16", 1, 40, 24576, 128, 1, 0), ("f32", 1, 40, 8192, 32, 0, 1),
+    ("bf16", 1, 40, 24576, 128, 1, 0), ("f32", 1, 40, 8192, 32, 0, 1), ("f32", 1, 40, 16384, 32, 0, 1), ("f32", 1, 40, 12288, 64, 1, 0),
     # chunks of rows, and more of them than the workspace holds at a time
     ("bf16", 49, 70, 256, 64, 1, 0), ("bf16", 160, 33, 1024, 128, 0, 1), ("f32", 200, 40, 14336, 128, 1, 0), ("bf16", 500, 17, 14336, 64, 0, 0),
     # so long that fewer column tiles go into the workspace
