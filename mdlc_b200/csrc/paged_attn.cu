@@ -35,8 +35,8 @@ constexpr int kUnit = 128;      // keys of one unit of split work
 constexpr int kTileCost = 2;
 constexpr int kMaxBlocks = 512; // split-mode blocks at most (bounds the workspace)
 constexpr int kJoinThreads = 256;
-constexpr int kLeastKeys = 256; // keys of a share of a chunk tile at least
-constexpr int kChunkBlocks = 148;  // shares are made until chunk mode fills this many SMs
+constexpr int kLeastKeys = 256; // keys of a share of a chunk tile at least, see splits_of
+constexpr int kB200Sms = 148;   // shares are made for so many SMs (the workspace's size is an answer without a context)
 
 template <typename T, int HDP>
 constexpr int block_keys() { return sizeof(T) * HDP <= 256 ? 32 : 16; }
@@ -945,7 +945,7 @@ size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 // chunk mode's geometry: which kernel, row tiles at most (full ones, and one more per request), shares per tile
 struct Chunk {
   bool used, tc;
-  int rows, tiles, splits;
+  int rows, tiles, splits, short_splits;
 };
 Chunk chunk_of(const mdlc_attn_desc& d) {
   const int group = d.heads / d.kv_heads;
@@ -954,11 +954,16 @@ Chunk chunk_of(const mdlc_attn_desc& d) {
   c.tc = attn_tc_fits(d) && (long long)d.tokens * group / attn_tc_rows(d.head_dim) + d.batch <= 65535;  // the tiles are its grid's y
   c.rows = c.tc ? attn_tc_rows(d.head_dim) : 64;
   c.tiles = (int)min((long long)d.tokens * group / c.rows + d.batch, (long long)INT32_MAX);
-  // blocks on an SM: two of one row tile, one of two. The mma.sync kernel's shares are made for four, of which two run at a time:
-  // `tiles` counts a part-filled tile more per request than there may be (fp32, five mixed requests: four 68 us, five 75,
-  // eight 79; twelve requests of up to 130 tokens: four 74, five 58)
-  const long long room = kChunkBlocks * (c.tc ? (c.rows == 128 ? 2 : 1) : 4) / ((long long)c.tiles * d.kv_heads);
-  c.splits = (int)max(1ll, min(room, min(16ll, (long long)d.max_kv / kLeastKeys)));
+  // Blocks on an SM: two of one row tile, one of two. The mma.sync kernel, of which two run at a time, has its shares made for twelve,
+  // so that the last blocks to end are short; for four where that would leave a share under 512 keys, since every share costs
+  // its part of the join. (`tiles` counts a part-filled tile more per request than there may be. Twenty fp32 batches of 1 to 24 requests of
+  // 30 to 700 tokens on 100 to 6000 keys: twelve within 3%; 24 requests of up to 200 tokens on 6000 keys 578 us for four,
+  // 441 for twelve, 24 mixed ones of 64 heads 750 and 594, 16 mixed ones on 4000 keys 165 and 99; five mixed ones on 1700 keys 66
+  // and 77, twelve of up to 130 tokens on 400 keys 62 and 66.)
+  const long long blocks = (long long)c.tiles * d.kv_heads;
+  auto shares = [&](int per_sm, int keys) { return (int)max(1ll, min(kB200Sms * per_sm / blocks, min(16ll, (long long)d.max_kv / keys))); };
+  c.short_splits = shares(c.tc ? (c.rows == 128 ? 2 : 1) : 4, kLeastKeys);
+  c.splits = c.tc ? c.short_splits : max(c.short_splits, shares(12, 2 * kLeastKeys));
   return c;
 }
 
@@ -1032,6 +1037,7 @@ bool narrow_fits(const mdlc_attn_desc& d) { return d.dtype == MDLC_BF16 && d.pag
 template <typename T, int HDP>
 cudaError_t run_chunks(mdlc_ctx* ctx, cudaStream_t stream, AttnArgs& a, const Chunk& c) {
   a.splits = c.splits;
+  a.short_splits = c.short_splits;
   mdlc_note_launch(ctx);
   cudaError_t e;
   if (c.tc) {

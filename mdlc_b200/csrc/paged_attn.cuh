@@ -23,7 +23,7 @@ struct AttnArgs {
   int group;          // query heads per key head
   SmallDiv group_div;
   int split_rows;     // requests with at most this many rows go to split mode
-  int splits;         // chunk mode: blocks that may share a row tile's keys
+  int splits, short_splits;  // chunk mode: blocks that may share a row tile's keys; the same where their shares are short
   float scale_log2;   // scale * log2(e)
   // workspace: partial sums [slot][rows][hdp], their maxima (base-2 exponent) and sums [slot][rows]
   float *part_o, *part_m, *part_l;
@@ -136,8 +136,10 @@ MDLC_DEV bool find_tile(const AttnArgs& a, long long want, int tile_rows, long l
   t->rows = t->rq.q_len * a.group;
   return true;
 }
-// blocks that share a tile of n key blocks: each gets at least two
-MDLC_DEV int splits_of(const AttnArgs& a, int n, int least) { return max(1, min(a.splits, n / least)); }
+// blocks that share a tile of n key blocks: each gets at least `least`, twice as many where more than short_splits share
+MDLC_DEV int splits_of(const AttnArgs& a, int n, int least) {
+  return max(1, max(min(a.short_splits, n / least), min(a.splits, n / (2 * least))));
+}
 
 template <typename T>
 MDLC_DEV void store_out(T* p, float v);
