@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page
     const int c = held_tok[b];
     const int held = (int)pages_of(c, pd), take = (int)pages_of((uint32_t)c + (uint32_t)(starts[b + 1] - starts[b]), pd) - held;
     for (int j = lane; j < take; j += 32)
-      p.table[(long long)b * d.table_stride + held + j] = __ldg(p.free_list + first[b] + j);
+      if (MDLC_CHECK_IDX(err, held + j, d.table_stride) && MDLC_CHECK_IDX(err, first[b] + j, d.free_pages)) p.table[(long long)b * d.table_stride + held + j] = __ldg(p.free_list + first[b] + j);
   }
 
   // slots and positions
@@ -170,6 +170,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const mdlc_page
       pos = c + (t - starts[lo]);
       if (first[lo] >= 0) {
         const int at = (int)page_index(pos, pd), held = (int)pages_of(c, pd);
+        if (!MDLC_CHECK_IDX(err, at < held ? at : first[lo] + (at - held), at < held ? d.table_stride : d.free_pages)) continue;
         // a page taken by this call comes from the free list itself: its table entry may not be written yet
         const int id = at < held ? __ldg(p.table + (long long)lo * d.table_stride + at)
                                  : __ldg(p.free_list + first[lo] + (at - held));
@@ -290,6 +291,8 @@ __global__ void __launch_bounds__(kRopeThreads, 5) rope_append_kernel(const Rope
   T* kc = static_cast<T*>(a.k_cache) + at;
   T* vc = static_cast<T*>(a.v_cache) + at;
   const int h1 = stored ? hr : d.heads;  // heads to write
+  // (the checked build: the last element of the token's last head)
+  if (stored && !MDLC_CHECK_IDX(err, at + (d.kv_heads - 1) * head_step + d.head_dim - 1, (long long)d.pages * d.kv_heads * head_step)) return;
   auto dst_of = [&](int h) { return h < d.heads ? qo + (long long)h * d.head_dim : kc + (h - d.heads) * head_step; };
 
   if (hl < lanes) {

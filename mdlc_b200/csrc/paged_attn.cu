@@ -193,6 +193,7 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
   auto id_of = [&](int blk) {
     const int j = base_of(blk) + lane;
     if (blk >= blk1 || lane >= BT || j >= rq.kv_len || (j < sp.lo && j >= d.sinks)) return kHiddenPage;
+    if (!table_ok(a, b, j / d.page)) return kHiddenPage;
     return max(__ldg(a.table + (long long)b * d.table_stride + j / d.page), kHiddenPage + 1);
   };
   // its cache row, or -1: hidden or missing
@@ -407,11 +408,13 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
     if (whole) {
       const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
       const int tok = rq.q0 + r / a.group, head = e * a.group + r % a.group;
+      if (!out_ok(a, tok, head, c, 4)) continue;
       T* po = static_cast<T*>(a.out) + (long long)tok * d.out_stride + (long long)head * d.head_dim + c;
       store_out<T>(po, acc.x * inv); store_out<T>(po + 1, acc.y * inv); store_out<T>(po + 2, acc.z * inv); store_out<T>(po + 3, acc.w * inv);
       if (a.lse && c == 0) a.lse[(long long)tok * d.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
     } else {
       const long long at = slot * K::ROWS + rl;
+      if (!part_ok(a, at)) continue;
       *reinterpret_cast<float4*>(a.part_o + at * HDP + c) = acc;
       if (c == 0) {
         a.part_m[at] = top;
@@ -455,6 +458,7 @@ MDLC_DEV void join_pieces(const AttnArgs& a, int b, int e, const Request& rq, in
 #pragma unroll 8
       for (int c = c0 + w; c <= c1; c += wpr) {
         const long long at = (slot0 + c) * ROWS + r;
+        if (!part_ok(a, at)) continue;
         const float pm = __ldcg(a.part_m + at), pl = __ldcg(a.part_l + at);
         float x[V];
 #pragma unroll
@@ -493,8 +497,8 @@ MDLC_DEV void join_pieces(const AttnArgs& a, int b, int e, const Request& rq, in
       T* po = static_cast<T*>(a.out) + (long long)tok * d.out_stride + (long long)head * d.head_dim;
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (i * 32 + lane < d.head_dim) store_out<T>(po + i * 32 + lane, acc[i] * inv);
-      if (a.lse && lane == 0) a.lse[(long long)tok * d.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
+        if (i * 32 + lane < d.head_dim && out_ok(a, tok, head, i * 32 + lane, 1)) store_out<T>(po + i * 32 + lane, acc[i] * inv);
+      if (a.lse && lane == 0 && out_ok(a, tok, head, 0, 1)) a.lse[(long long)tok * d.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
     }
   }
   __syncthreads();
@@ -660,6 +664,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
     auto id_of = [&](int blk) {
       const int k0 = key_of_block(sp, blk, BT) + my_page * box;
       if (blk >= blk1 || !mine || k0 >= sp.hi || (k0 + box <= sp.lo && k0 >= d.sinks)) return kHiddenPage;
+      if (!table_ok(a, b, k0 >> page_log2)) return kHiddenPage;
       return max(__ldg(a.table + (long long)b * d.table_stride + (k0 >> page_log2)), kHiddenPage + 1);
     };
     // its cache row, or one past the maps: hidden or missing
@@ -845,6 +850,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
       if (whole) {
         const float inv = sum > 0.0f ? 1.0f / sum : (sum == 0.0f ? 0.0f : sum);
         const int tok = rq.q0 + rl / a.group, head = e * a.group + rl % a.group;
+        if (!out_ok(a, tok, head, c, 4)) continue;
         uint2 v;
         v.x = pack_bf16x2(acc.x * inv, acc.y * inv);
         v.y = pack_bf16x2(acc.z * inv, acc.w * inv);
@@ -852,6 +858,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
         if (a.lse && c == 0) a.lse[(long long)tok * d.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
       } else {
         const long long at = slot * C::ROWS + rl;
+        if (!part_ok(a, at)) continue;
         *reinterpret_cast<float4*>(a.part_o + at * HDP + c) = acc;
         if (c == 0) {
           a.part_m[at] = top;
@@ -905,6 +912,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_chunk_join_kernel(const Att
   const int per = (tile_rows + gridDim.z - 1) / gridDim.z, rl0 = blockIdx.z * per;
   for (int rl = rl0 + warp; rl < min(rl0 + per, min(tile_rows, t.rows - t.r0)); rl += kJoinThreads / 32) {
     const int r = t.r0 + rl;
+    if (!part_ok(a, (slot0 + ns - 1) * tile_rows + rl)) continue;
     float top = -INFINITY, sum = 0.0f, acc[V] = {};
     for (int s = 0; s < ns; ++s) top = fmaxf(top, a.part_m[(slot0 + s) * tile_rows + rl]);
     const float safe = top == -INFINITY ? 0.0f : top;
@@ -921,8 +929,8 @@ __global__ void __launch_bounds__(kJoinThreads) attn_chunk_join_kernel(const Att
     T* po = static_cast<T*>(a.out) + (long long)tok * d.out_stride + (long long)head * d.head_dim;
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i * 32 + lane < d.head_dim) store_out<T>(po + i * 32 + lane, acc[i] * inv);
-    if (a.lse && lane == 0) a.lse[(long long)tok * d.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
+      if (i * 32 + lane < d.head_dim && out_ok(a, tok, head, i * 32 + lane, 1)) store_out<T>(po + i * 32 + lane, acc[i] * inv);
+    if (a.lse && lane == 0 && out_ok(a, tok, head, 0, 1)) a.lse[(long long)tok * d.heads + head] = (top + log2f(sum)) * 0.69314718055994531f;
   }
 }
 
@@ -969,7 +977,7 @@ Chunk chunk_of(const mdlc_attn_desc& d) {
 
 // partial sums, maxima and sums of split mode's slots, then chunk mode's (the two run side by side)
 struct Layout {
-  size_t o[2], m[2], l[2], total;
+  size_t rows[2], o[2], m[2], l[2], total;
 };
 Layout layout_of(const mdlc_attn_desc& d) {
   const Chunk c = chunk_of(d);
@@ -977,6 +985,7 @@ Layout layout_of(const mdlc_attn_desc& d) {
                           c.used && c.splits > 1 ? (size_t)c.tiles * d.kv_heads * c.splits * c.rows : 0};
   Layout l = {};
   for (int i = 0; i < 2; ++i) {
+    l.rows[i] = rows[i];
     l.o[i] = l.total;
     l.m[i] = l.o[i] + align256(rows[i] * padded_dim(d.head_dim) * 4);
     l.l[i] = l.m[i] + align256(rows[i] * 4);
@@ -1119,6 +1128,7 @@ extern "C" int mdlc_paged_attn(mdlc_ctx* ctx, const mdlc_attn_desc* desc, const 
   a.group = desc->heads / desc->kv_heads;
   a.group_div = small_div(a.group);
   a.split_rows = 16 * split_groups(*desc);
+  a.err = ctx->d_err;
   a.scale_log2 = desc->scale * 1.4426950408889634f;
   const Layout l = layout_of(*desc);
   char* ws = static_cast<char*>(workspace);
@@ -1126,6 +1136,7 @@ extern "C" int mdlc_paged_attn(mdlc_ctx* ctx, const mdlc_attn_desc* desc, const 
     a.part_o = reinterpret_cast<float*>(ws + l.o[mode]);
     a.part_m = reinterpret_cast<float*>(ws + l.m[mode]);
     a.part_l = reinterpret_cast<float*>(ws + l.l[mode]);
+    a.part_rows = (long long)l.rows[mode];
   };
   place(0);
   AttnArgs split = a;

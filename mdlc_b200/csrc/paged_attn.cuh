@@ -27,6 +27,8 @@ struct AttnArgs {
   float scale_log2;   // scale * log2(e)
   // workspace: partial sums [slot][rows][hdp], their maxima (base-2 exponent) and sums [slot][rows]
   float *part_o, *part_m, *part_l;
+  long long part_rows;    // rows of the workspace, and the error word: for the checked build
+  int* err;
   int* arrived;           // split mode: arrivals at the tile that starts in block c and others share
 };
 
@@ -73,6 +75,16 @@ MDLC_DEV Span span_of(const AttnArgs& a, const Request& r, int i0, int i1, int b
 MDLC_DEV int key_of_block(const Span& s, int blk, int bt) {
   return blk < s.n_first ? blk * bt : s.start + (blk - s.n_first) * bt;
 }
+
+// ------------------------------------------------------------ index checks (constant true but in the checked build)
+MDLC_DEV bool table_ok(const AttnArgs& a, int b, int entry) {
+  return MDLC_CHECK_IDX(a.err, b, a.d.batch) && MDLC_CHECK_IDX(a.err, entry, a.d.table_stride);
+}
+// columns [c, c + n) of a head of a token
+MDLC_DEV bool out_ok(const AttnArgs& a, long long tok, int head, int c, int n) {
+  return MDLC_CHECK_IDX(a.err, tok, a.d.tokens) && MDLC_CHECK_IDX(a.err, head, a.d.heads) && MDLC_CHECK_IDX(a.err, c + n - 1, a.d.head_dim);
+}
+MDLC_DEV bool part_ok(const AttnArgs& a, long long row) { return MDLC_CHECK_IDX(a.err, row, a.part_rows); }
 
 // ------------------------------------------------------------ finding work
 // exclusive sum over the block's threads of v; *total: the sum of all

@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
     // Ids that do not exist hide their keys: looked for once, so that the blocks need not look (a load from the table
     // in front of every block cost 570 cycles of 4200)
     auto missing = [&](int j) {
-      return j < sp.hi && (j + min(d.page, kKeys) > sp.lo || j < d.sinks) &&
+      return j < sp.hi && (j + min(d.page, kKeys) > sp.lo || j < d.sinks) && table_ok(a, t.b, j >> page_log2) &&
              (unsigned)__ldg(a.table + (long long)t.b * d.table_stride + (j >> page_log2)) >= (unsigned)d.pages;
     };
     {
@@ -414,23 +414,24 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
             if (t.r0 + rw < t.rows && 8 * k < d.head_dim) {
               int head;
               const int tok = token_of(rw, &head);
+              if (!out_ok(a, tok, head, 8 * k, 8)) continue;
               *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + tok * d.out_stride + (long long)head * d.head_dim + 8 * k) =
                   *reinterpret_cast<const uint4*>(rows + row * HDP * 2 + ((k ^ (row & 7)) << 4));
             }
           }
-        } else if (live) {
+        } else if (live && part_ok(a, slot)) {
 #pragma unroll
           for (int k = 0; k < HDP; k += 4)
             *reinterpret_cast<uint4*>(a.part_o + slot * HDP + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
         }
         if (live) {
-          if (ns > 1) {
+          if (ns > 1 && part_ok(a, slot)) {
             a.part_m[slot] = mlog;
             a.part_l[slot] = l;
-          } else if (a.lse) {
+          } else if (ns == 1 && a.lse) {
             int head;
             const long long tok = token_of(rl, &head);
-            a.lse[tok * d.heads + head] = (mlog + log2f(l)) * 0.69314718055994531f;
+            if (out_ok(a, tok, head, 0, 1)) a.lse[tok * d.heads + head] = (mlog + log2f(l)) * 0.69314718055994531f;
           }
         }
       }
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
       const int k0 = base + page_i * box;
       int row = none;
       if (mine && k0 < sp.hi && (k0 + box > sp.lo || k0 < d.sinks)) {
-        const int id = __ldg(a.table + (long long)t.b * d.table_stride + k0 / d.page);
+        const int id = table_ok(a, t.b, k0 / d.page) ? __ldg(a.table + (long long)t.b * d.table_stride + k0 / d.page) : -1;
         if ((unsigned)id < (unsigned)d.pages) row = (id * d.kv_heads + e) * d.page + k0 % d.page;
         else record_error(err, MDLC_DEVERR_BOUNDS);
       }

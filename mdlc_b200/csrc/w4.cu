@@ -123,7 +123,7 @@ MDLC_DEV void x_unit(const W4Args& a, const uint4 (&raw)[2], int u, int col0, ui
 template <bool BF16>
 MDLC_DEV void x_load(const W4Args& a, int row, int u, bool ok, uint4 (&raw)[2]) {
   raw[0] = raw[1] = make_uint4(0, 0, 0, 0);
-  if (!ok) return;
+  if (!ok || !MDLC_CHECK_IDX(a.err, row, a.d.m) || !MDLC_CHECK_IDX(a.err, u * 8 + 7, a.d.k)) return;
   const long long at = (long long)row * a.d.x_stride + u * 8;
   if (BF16) {
     raw[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.x) + at));
@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(128) w4_parts_kernel(const W4Args a, uint8_t* 
   uint4 raw[2];
   x_load<BF16>(a, row, u, u < a.d.k / 8, raw);
   const int chunk = row / a.rows_per_chunk;
+  if (!MDLC_CHECK_IDX(a.err, ((long long)chunk * steps + u / 16 + 1) * a.step_bytes - 1, kSplitWsBytes)) return;
   x_unit<BF16>(a, raw, u, a.parts * (row - chunk * a.rows_per_chunk), ready + ((long long)chunk * steps + u / 16) * a.step_bytes);
 }
 
@@ -212,7 +213,8 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) cp_async_16_all(dst + (r * 2 + h) * (kW4Warps * 32 * 16), wp[r][h] + (uint32_t)w_step * 64);
+        for (int h = 0; h < 2; ++h)
+          if (MDLC_CHECK_IDX(a.err, wp[r][h] + (uint32_t)w_step * 64 + 15 - a.codes, (long long)d.n * half)) cp_async_16_all(dst + (r * 2 + h) * (kW4Warps * 32 * 16), wp[r][h] + (uint32_t)w_step * 64);
     }
     cp_async_commit();
     w_step += kW4Warps;
@@ -247,6 +249,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
         for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            if (!MDLC_CHECK_IDX(a.err, sp[r][h] - a.scales + min(grp, groups - 1), (long long)d.n * groups)) continue;
             sc_next[i][r][h] = G128 || grp < groups ? __ldg(sp[r][h] + grp) : 0;
             if (ZEROS) zr_next[i][r][h] = G128 || grp < groups ? __ldg(zp[r][h] + grp) : 0;
           }
@@ -399,6 +402,7 @@ __global__ void __launch_bounds__(kW4Warps * 32, w4_min_blocks<NT, R>()) gemv_w4
         v *= kCodeUnit;
         if (a.bias) v += __ldg(a.bias + n);
         const long long at = (long long)(m0 + xr) * d.y_stride + n;
+        if (!MDLC_CHECK_IDX(a.err, m0 + xr, d.m)) continue;
         if (d.y_type == MDLC_BF16) static_cast<__nv_bfloat16*>(a.y)[at] = __float2bfloat16_rn(v);
         else static_cast<float*>(a.y)[at] = v;
       }
