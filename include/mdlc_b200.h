@@ -456,8 +456,8 @@ int mdlc_rope_append(mdlc_ctx* ctx, const mdlc_rope_desc* desc, const void* q, c
                      void* v_cache);
 
 /* Attention of each request's new tokens over its cache pages. With i the
- * token's index among its request's q_len new ones, it stands at position
- * p = kv_lens[b] - q_len + i and sees key j when
+ * token's index among its request's q_len = q_starts[b + 1] - q_starts[b] new ones, it
+ * stands at position p = kv_lens[b] - q_len + i and sees key j when
  *   j <= p and (window == 0 or j > p - window or j < sinks),
  *   out = sum_j exp(s_j - lse) v_j,  s_j = scale q . k_j,  lse = log sum_j exp(s_j);
  * a token that sees no key gets out = 0, lse = -inf. Heads e * G .. e * G + G - 1
@@ -471,8 +471,10 @@ int mdlc_rope_append(mdlc_ctx* ctx, const mdlc_rope_desc* desc, const void* q, c
  * it (as 0 x inf). Rows past q_starts[batch] are left
  * as they are. `workspace`: mdlc_paged_attn_workspace bytes, 16-byte aligned, for
  * this call alone. q, out and caches are 16-byte aligned, the strides multiples of 8
- * elements. max_q and max_kv bound every request's q_len and kv_len: longer ones
- * are cut to them (kv_len also to table_stride * page). */
+ * elements. max_q and max_kv bound every request's q_len and kv_len. Of a request
+ * with more tokens the first max_q are computed, where they stand, and the others' rows left as
+ * they are (as are rows past `tokens`); a longer kv_len counts as max_kv (and as
+ * table_stride * page at most). */
 typedef struct {
   int32_t batch;   /* 1 .. MDLC_MAX_REQUESTS */
   int32_t tokens;  /* rows of q and out */

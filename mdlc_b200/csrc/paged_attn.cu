@@ -141,7 +141,7 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
   const uint32_t ring = smem_u32(smem) + wn * kStages * K::STAGE;
   const int chunks = d.head_dim / EC;
   const int rows = rq.q_len * a.group;
-  const int shift = rq.kv_len - rq.q_len;
+  const int shift = rq.shift;
   auto sync_group = [&]() {
     if constexpr (WM == 1) __syncwarp(); else named_sync(1 + wn, GT);
   };
@@ -154,7 +154,7 @@ MDLC_DEV void attn_piece(const AttnArgs& a, unsigned char* smem, uint32_t (*vali
     const int r = r0 + wm * 16 + h * 8 + g;
     const bool ok = r < rows;
     const int i = ok ? r / a.group : 0;
-    pos[h] = ok ? shift + i : -1;
+    pos[h] = ok ? max(-1, shift + i) : -1;
     qp[h] = ok ? static_cast<const T*>(a.q) + (long long)(rq.q0 + i) * d.q_stride + (long long)(e * a.group + r % a.group) * d.head_dim : nullptr;
   }
   constexpr int KS = kBf16 ? HDP / 16 : HDP / 8;  // steps of the score product
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
   uint32_t begun = 0, used = 0;  // blocks issued and consumed by this warp so far
 
   auto piece = [&](int b, const Request& rq, int e, const Span& sp, int blk0, int blk1, bool whole, long long slot) {
-    const int rows = rq.q_len * a.group, shift = rq.kv_len - rq.q_len;
+    const int rows = rq.q_len * a.group, shift = rq.shift;
     // queries as the column operand: row 8 n + g, columns 16 ks + 2 t and + 8
     uint32_t qb[MT][NT][2];
     int pos[NT][2];  // positions of this thread's result columns, rows 8 n + 2 t and + 1
@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_narrow_kernel(const Attn
           qb[ks][n][i] = (r < rows && c < d.head_dim) ? __ldg(reinterpret_cast<const uint32_t*>(qp + c)) : 0u;
         }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) pos[n][i] = 8 * n + 2 * t + i < rows ? shift + (8 * n + 2 * t + i) / a.group : -1;
+      for (int i = 0; i < 2; ++i) pos[n][i] = 8 * n + 2 * t + i < rows ? max(-1, shift + (8 * n + 2 * t + i) / a.group) : -1;
     }
     // page id of this lane's box, kHiddenPage: hidden from every row. Loads only, so that several are in flight.
     auto id_of = [&](int blk) {

@@ -44,6 +44,7 @@ cudaError_t attn_tensor_maps(const AttnArgs& a, int box, CUtensorMap* k, CUtenso
 // ------------------------------------------------------------ one request's geometry
 struct Request {
   int q0, q_len, kv_len;
+  int shift;  // position of row 0; q_len may be fewer rows than the request has (max_q, tokens), the positions are those of all
 };
 MDLC_DEV Request request_of(const AttnArgs& a, int b) {
   Request r;
@@ -51,6 +52,7 @@ MDLC_DEV Request request_of(const AttnArgs& a, int b) {
   r.q0 = max(0, min(s0, a.d.tokens));
   r.q_len = min(max(0, min(s1, a.d.tokens) - r.q0), a.d.max_q);
   r.kv_len = max(0, min(__ldg(a.kv_lens + b), a.d.max_kv));  // the host has cut max_kv to the table's row
+  r.shift = r.kv_len - max(0, s1 - r.q0);
   return r;
 }
 
@@ -62,9 +64,8 @@ struct Span {
 };
 MDLC_DEV Span span_of(const AttnArgs& a, const Request& r, int i0, int i1, int bt) {
   Span s;
-  const int shift = r.kv_len - r.q_len;
-  s.hi = max(0, min(r.kv_len, shift + i1 + 1));
-  s.lo = a.d.window > 0 ? (int)max(0ll, (long long)shift + i0 - a.d.window + 1) : 0;
+  s.hi = max(0, min(r.kv_len, r.shift + i1 + 1));
+  s.lo = a.d.window > 0 ? (int)max(0ll, (long long)r.shift + i0 - a.d.window + 1) : 0;
   s.n_first = (min(a.d.sinks, s.lo) + bt - 1) / bt;
   s.start = s.lo / bt * bt;
   if (s.start <= s.n_first * bt) s.n_first = s.start = 0;

@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
   const int ns = splits_of(a, sp.n, 2);
   if ((int)blockIdx.z >= ns) return;
   const int blk0 = (int)((long long)blockIdx.z * sp.n / ns), blk1 = (int)((long long)(blockIdx.z + 1) * sp.n / ns), nb = blk1 - blk0;
-  const int shift = t.rq.kv_len - t.rq.q_len;
+  const int shift = t.rq.shift;
   const int n_tiles = C::TILES == 2 && t.rows - t.r0 > 128 ? 2 : 1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRing; ++i) mbar_init(bar(kEmpty + i), n_tiles);  // both tiles' MMAs give a key or value tile back
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(TcCfg<HDP>::THREADS, 3 - TcCfg<HDP>::TILES) at
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_addr = tmem + lanes + tile * 128, o_addr = tmem + lanes + C::O_COL + tile * HDP;
     const bool live = r < t.rows;
-    const int p = live ? shift + r / a.group : -1;
+    const int p = live ? max(-1, shift + r / a.group) : -1;
     const int first = t.r0 + tile * 128, last = min(first + 127, t.rows - 1);
     const int p_min = shift + first / a.group, p_max = shift + last / a.group;
     const float c = a.scale_log2;
