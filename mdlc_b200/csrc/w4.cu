@@ -9,8 +9,8 @@
 //   * x is the 8-column operand: a bf16 row is one column as it is, an fp32 row three, whose sum it is exactly (8 bits each, cut
 //     off in turn; below 2^-110 the last bits go). No scale is shared between columns of x, so a large one that meets weights of
 //     zero takes nothing from its neighbours. (Fixed-point digits with a shared scale on the int8 pipe cost three operations for
-//     eight codes - one row of 65536 x 8192 55 us, here 67 us, 4.1 TB/s - but an error that followed the largest |x| of 128
-//     columns, and three columns for a bf16 row too: 16 rows of 14336 x 4096 51 us, here 33 us.)
+//     eight codes - one row of 65536 x 8192 55-59 us, here 68-73 us, 3.8-4.1 TB/s - but an error that followed the largest |x| of 128
+//     columns, and three columns for a bf16 row too: 16 rows of 14336 x 4096 51 us, here 34 us.)
 //   * a group is summed from zero in the tensor core, scaled and added to the row's fp32 sum.
 // The order of the columns inside a product is free as long as both operands agree, so a thread keeps
 // the 32 consecutive codes of its 16-byte load. For groups under 128 columns the four threads of a row hold different
@@ -458,7 +458,8 @@ cudaError_t launch_w4(mdlc_ctx* ctx, W4Args& a, const W4Plan& p) {
   };
   if (a.d.group == 128) return a.zeros ? go(0, gemv_w4_kernel<NT, R, 128, true>) : go(1, gemv_w4_kernel<NT, R, 128, false>);
   if (a.d.group == 64) return a.zeros ? go(2, gemv_w4_kernel<NT, R, 64, true>) : go(3, gemv_w4_kernel<NT, R, 64, false>);
-  return a.zeros ? go(4, gemv_w4_kernel<NT, R, 32, true>) : go(5, gemv_w4_kernel<NT, R, 32, false>);
+  if constexpr (R == 1) return a.zeros ? go(4, gemv_w4_kernel<NT, R, 32, true>) : go(5, gemv_w4_kernel<NT, R, 32, false>);
+  return cudaErrorInvalidValue;  // groups of 32 take one row tile
 }
 
 template <int NT>
@@ -475,8 +476,10 @@ cudaError_t launch_w4_cols(mdlc_ctx* ctx, W4Args& a) {
   const int m = a.d.m, batch = ready ? (int)min((long long)m, fit * a.rows_per_chunk) : m;
   const W4Plan one = w4_plan<NT, 1>(a, ctx->num_sms), two = w4_plan<NT, 2>(a, ctx->num_sms);
   // Two row tiles share a read of x: a round of them takes less than two of single ones. The fewer and fuller
-  // rounds win (65536 rows: 7 rounds of two tiles 67 us; 4096 rows: one round either way).
-  const bool pair = two.span && (!one.span || 3 * two.rounds() < 2 * one.rounds());
+  // rounds win (one row of 65536 x 8192: 7 rounds of two tiles 68 us, 14 of one 80; 24 rows of 28672 x 4096: 78 and 98; 4096 outputs: one round
+  // either way), but for groups of 32, whose scales take the registers of a second tile (one row of 14336 x 4096: two tiles 33 us, one 27;
+  // 8 rows of 4096 x 14336: 36 and 33).
+  const bool pair = a.d.group > 32 && two.span && (!one.span || 3 * two.rounds() < 2 * one.rounds());
   for (int m0 = 0; m0 < m; m0 += batch) {
     W4Args b = a;
     b.d.m = min(batch, m - m0);
