@@ -196,7 +196,12 @@ int mdlc_get_stream(mdlc_ctx* ctx, void** stream); /* cudaStream_t of the contex
  * default stream). The new stream first waits for what the context has issued
  * so far. The caller's stream must outlive its use here: unbind (which makes the
  * own stream wait in the same way) or bind another before destroying it.
- * Rejected while a graph is being captured. */
+ * Rejected while a graph is being captured by mdlc_graph_begin.
+ * A context's work runs one call after the other: its scratch memory (partial sums
+ * and counters of split-K products, the split x of mdlc_gemv_w4, arrivals and the
+ * side stream of mdlc_paged_attn) serves one call at a time. A graph that a caller
+ * captured from a bound stream is the context's work too: order its replays with
+ * everything else of the context, or give it a context of its own. */
 int mdlc_bind_stream(mdlc_ctx* ctx, void* stream);
 int mdlc_unbind_stream(mdlc_ctx* ctx);
 
@@ -393,8 +398,8 @@ int mdlc_se_fc(mdlc_ctx* ctx, const mdlc_se_desc* desc, const void* pooled, cons
  * its cache pages the ids in row b of a block table [batch][table_stride].
  * Lengths, tables and slots live on the device and are read by the kernels, so a
  * captured step replays with new ones; the host gives upper bounds. Ids, slots
- * and positions read on the device are checked: one outside its range is
- * skipped and records MDLC_DEVERR_BOUNDS in the error word. */
+ * and positions read on the device are checked: what one outside its range stands
+ * for is skipped, and MDLC_DEVERR_BOUNDS recorded in the error word. */
 #define MDLC_MAX_REQUESTS 8192
 
 /* Block tables, slot maps and positions from request lengths. Request b holds
@@ -405,7 +410,8 @@ int mdlc_se_fc(mdlc_ctx* ctx, const mdlc_se_desc* desc, const void* pooled, cons
  * entries are left as they are. A request that would need more than
  * table_stride entries or more pages than are left is refused: its row keeps its
  * entries, its slots are -1 and kv_lens[b] stays cached_lens[b] (the pages that
- * it would have taken are then not given to later requests either).
+ * it would have taken are then not given to later requests either), and its rows
+ * mean nothing in an attention that follows.
  * New tokens that have no row, past the first `tokens` of all, are not planned: a
  * request counts as if it brought only those that have one.
  * q_starts[batch + 1]: running sums of new_lens, at most `tokens`; kv_lens[b]
@@ -438,8 +444,9 @@ int mdlc_page_plan(mdlc_ctx* ctx, const mdlc_page_desc* desc, const int32_t* cac
  * [0, max_pos); table: [max_pos][rot_dim / 2][2] fp32. q, k, v and q_out hold
  * [tokens][heads][head_dim] with a stride between tokens each (slices of one
  * packed projection, for instance); q_out may be q itself. A token whose slot is
- * negative is padding: its q_out is written, the caches are not. q_out null:
- * only the caches are written. */
+ * negative is padding: its q_out is written, the caches are not; the same for one
+ * past the caches. A token with a position outside [0, max_pos) on any axis is
+ * skipped whole: query, key and value. q_out null: only the caches are written. */
 typedef struct {
   int32_t tokens, heads, kv_heads, head_dim;
   int32_t rot_dim;     /* even, <= head_dim */
